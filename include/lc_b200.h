@@ -301,6 +301,84 @@ lcError_t lcMatrixDiv(const void* a, const void* b, void* out, size_t rows, size
  * (the reference's LN formula, README.md:2267-2270).  Device pointers, fp32. */
 lcError_t lcLayerNorm(const float* x, float* out, size_t rows, size_t cols, float eps, lcStream_t stream);
 
+/* ---- the cross-attention layer of an encoder-decoder: no counterpart in the reference --------
+ * Layer norm with weights (forward, and backward with the weights' gradients), and attention of
+ * the decoder's queries over an encoder's keys and values (forward, its form for a few tokens,
+ * and backward). */
+
+/* out = (x - mean) * rstd * gamma + beta over the last axis of [rows, cols], mean and rstd =
+ * 1/sqrt(var + eps) of each row (population variance), as lcLayerNorm with weights.  Device pointers,
+ * asynchronous on `stream`.  dtype (f32 or bf16) is x's and out's, param_dtype (f32 or bf16)
+ * gamma's and beta's; statistics and arithmetic are fp32 and `out` is rounded once.  gamma and beta
+ * (each [cols]) may be NULL: 1 and 0.  mean and rstd ([rows], fp32) receive what the backward pass
+ * needs; each may be NULL.  x_stride / out_stride are elements from row to row, 0 = cols (dense);
+ * a stride below cols is LC_INVALID_VALUE, as is an eps that is negative or NaN.  `out` may be x
+ * itself (with the same stride) and must not overlap it otherwise. */
+lcError_t lcLayerNormForward(const void* x, const void* gamma, const void* beta, void* out, float* mean, float* rstd,
+                             size_t rows, size_t cols, size_t x_stride, size_t out_stride, float eps,
+                             lcDataType dtype, lcDataType param_dtype, lcStream_t stream);
+
+/* Gradients of lcLayerNormForward, from dout, x, gamma and the forward's mean and rstd:
+ *   dx = rstd * (w - avg(w) - h * avg(w * h)) with h = (x - mean) * rstd, w = dout * gamma
+ *   dgamma[c] = sum over rows of dout * h,  dbeta[c] = sum over rows of dout
+ * dx (dtype) and dgamma / dbeta (param_dtype, overwritten) may each be NULL, but not all three;
+ * gamma NULL = 1.  The sums over rows are fp32 in a fixed order: the same call gives the same bits.
+ * dx may be dout or x itself (with the same stride) and must not overlap them otherwise.  Device
+ * pointers, asynchronous on `stream`; strides as above.  Allocates a stream-ordered workspace when
+ * dgamma or dbeta is wanted. */
+lcError_t lcLayerNormBackward(const void* dout, const void* x, const void* gamma, const float* mean,
+                              const float* rstd, void* dx, void* dgamma, void* dbeta, size_t rows, size_t cols,
+                              size_t dout_stride, size_t x_stride, size_t dx_stride, lcDataType dtype,
+                              lcDataType param_dtype, lcStream_t stream);
+
+/* Elements from one batch entry, head and token to the next; the head_dim values of a token and head
+ * are contiguous.  All three 0: dense [batch, heads, len, head_dim].  E.g. tensors as a projection
+ * leaves them, [batch, len, heads, head_dim]: {len*heads*head_dim, head_dim, heads*head_dim}. */
+typedef struct lcHeadStrides { size_t batch, head, token; } lcHeadStrides;
+
+/* One cross-attention problem.  q_heads is a multiple of kv_heads: query head h reads key head
+ * h / (q_heads / kv_heads).  All pointers are optional (NULL) int32 / byte arrays:
+ *   q_lens [batch]    queries of a batch entry; rows at or past it are not computed and every output
+ *                     keeps what it held there (out, lse, dq); they add nothing to dk and dv
+ *   kv_lens [batch]   keys of a batch entry; keys at or past it are masked
+ *   key_mask [batch, kv_len]   0 = masked, anything else = visible
+ * Lengths outside [0, q_len] / [0, kv_len] are clamped.  Masked keys and values are never used,
+ * whatever they hold (NaN and infinities included). */
+typedef struct lcCrossAttentionDesc {
+  size_t batch, q_heads, kv_heads, q_len, kv_len, head_dim;
+  lcHeadStrides q, k, v, out;
+  const int32_t* q_lens;
+  const int32_t* kv_lens;
+  const uint8_t* key_mask;
+  float scale; /* of the scores; 0 = 1/sqrt(head_dim) */
+  lcDataType dtype;
+} lcCrossAttentionDesc;
+
+/* out = softmax(scale * q k^T over the visible keys) v, the attention of lcAttentionForward for
+ * queries and keys of different lengths, shared key heads, strides and masks.  A row without a visible
+ * key is 0.  lse (fp32, dense [batch, q_heads, q_len], may be NULL) receives the log of each row's
+ * sum of exp(scale * q k^T) (-infinity for a row without a visible key), which the backward pass needs.
+ * f32: strict fp32 arithmetic; bf16: fp32 accumulation and softmax statistics; head_dim <= 256.
+ * k and v may be broadcast over the batch (batch stride 0 with the other strides set: one source
+ * for many targets).  `out` must not overlap itself or the inputs.
+ * Policy as lcAttentionForward (NULL: device pointers, asynchronous; the output postprocess must be
+ * neutral).  Host tensors are dense; q_lens follows upload_q, kv_lens and key_mask follow
+ * upload_k, lse follows download_out.  Few queries over many keys are split along the keys, with a
+ * stream-ordered workspace. */
+lcError_t lcCrossAttentionForward(const lcCrossAttentionDesc* desc, const void* q, const void* k, const void* v,
+                                  void* out, float* lse, const lcAttentionIoPolicy* policy, lcStream_t stream);
+
+/* Gradients of lcCrossAttentionForward from dout (laid out as out), the inputs, and the forward's
+ * out and lse: dq, dk, dv are laid out as q, k, v.  dq may be NULL, and dk and dv may both be NULL
+ * (not all three).  dk and dv are written for every key (0 for masked ones) and sum over the query
+ * heads of a key head and, when k and v are both broadcast over the batch, over the batch (one
+ * [kv_heads, kv_len, head_dim] gradient); the other strides that would make two gradients share memory
+ * are LC_INVALID_VALUE.  All sums are fp32 (or wider) in a fixed order: the same call gives the same
+ * bits.  Device pointers, asynchronous on `stream`; allocates a stream-ordered workspace. */
+lcError_t lcCrossAttentionBackward(const lcCrossAttentionDesc* desc, const void* dout, const void* q, const void* k,
+                                   const void* v, const void* out, const float* lse, void* dq, void* dk, void* dv,
+                                   lcStream_t stream);
+
 /* ---- device-resident sessions ----------------------------------------------------------------
  * AttentionSession (include/lightning_core/core/attention.hpp:86-129, src/attention.cpp:247-343) and
  * MatMulMetalResidentSession (include/lightning_core/core/ops.hpp:1339-1379): a handle bound to one

@@ -1,0 +1,30 @@
+// What the cross-attention kernels share.
+#pragma once
+
+#include "lc_internal.hpp"
+
+namespace lcb {
+
+// Length of a batch entry, clamped to what the tensors hold.
+__device__ __forceinline__ int cross_len(const int* lens, int b, int most) {
+  return lens ? min(max(lens[b], 0), most) : most;
+}
+
+// Parts of a forward pass that is split along the keys: part i of row r (rows are dense
+// [batch, q_heads, q_len]) holds the unnormalised sum o[i][r][.] of exp2(s - m) v over its keys and
+// ml[i][r] = (m, sum of exp2(s - m)), m the part's maximum of the scores in the log2 domain.
+struct CrossSplit {
+  int splits;
+  long long rows;
+  float* o;
+  float2* ml;
+};
+
+struct CrossSplitWork {
+  CrossSplit sp{};
+  void* ws = nullptr;
+  cudaError_t begin(const CrossArgs& a, long long blocks, int tile, cudaStream_t s);
+  cudaError_t end(const CrossArgs& a, cudaError_t launched, cudaStream_t s);
+};
+
+}  // namespace lcb

@@ -176,4 +176,47 @@ cudaError_t vector_add_f64(const double* a, const double* b, double* out, size_t
 cudaError_t matrix_binary(int op, int f64, const void* a, const void* b, void* out, size_t n, cudaStream_t s);
 cudaError_t layer_norm_f32(const float* x, float* out, size_t rows, size_t cols, float eps, cudaStream_t s);
 
+// ---- layer norm with weights (layer_norm.cu) --------------------------------------------------
+struct LayerNormArgs {
+  const void *x, *gamma, *beta;  // gamma, beta optional
+  void* out;
+  float *mean, *rstd;  // optional
+  size_t rows, cols, x_stride, out_stride;
+  float eps;
+  int bf16, param_bf16;
+};
+cudaError_t layer_norm_forward(const LayerNormArgs& a, cudaStream_t s);
+struct LayerNormGradArgs {
+  const void *dout, *x, *gamma;
+  const float *mean, *rstd;
+  void *dx, *dgamma, *dbeta;  // each optional
+  size_t rows, cols, dout_stride, x_stride, dx_stride;
+  int bf16, param_bf16;
+};
+cudaError_t layer_norm_backward(const LayerNormGradArgs& a, cudaStream_t s);
+
+// ---- cross attention (cross_attention*.cu) ----------------------------------------------------
+struct HeadStrides {
+  long long b, h, t;  // elements from one batch entry / head / token to the next
+};
+struct CrossArgs {
+  const void *q, *k, *v;
+  void* out;   // forward: written; backward: the forward's output, read
+  float* lse;  // dense [batch, hq, q_len]; forward: optional, written; backward: read
+  HeadStrides qs, ks, vs, os;
+  const int *q_lens, *kv_lens;
+  const unsigned char* key_mask;
+  int batch, hq, hk, q_len, kv_len, d;
+  float scale;
+  int bf16;
+};
+struct CrossGradArgs {
+  CrossArgs f;
+  const void* dout;  // laid out as out
+  void *dq, *dk, *dv;  // laid out as q, k, v; dq optional, dk and dv optional together
+  int kv_shared;  // k and v are broadcast over the batch: dk and dv sum over it
+};
+cudaError_t cross_attention_forward(const CrossArgs& a, cudaStream_t s);
+cudaError_t cross_attention_backward(const CrossGradArgs& a, cudaStream_t s);
+
 }  // namespace lcb

@@ -9,6 +9,7 @@
 #include <cmath>
 #include <cstring>
 #include <string>
+#include <utility>
 #include <vector>
 
 #include "lc_host.hpp"
@@ -753,6 +754,196 @@ lcError_t lcVectorAdd(const void* a, const void* b, void* out, size_t n, lcDataT
 lcError_t lcLayerNorm(const float* x, float* out, size_t rows, size_t cols, float eps, lcStream_t stream) {
   if (!x || !out || rows == 0 || cols == 0) return LC_INVALID_VALUE;
   LC_TRY(layer_norm_f32(x, out, rows, cols, eps, static_cast<cudaStream_t>(stream)));
+  return LC_SUCCESS;
+}
+
+static bool float_type(lcDataType t) { return t == LC_DTYPE_F32 || t == LC_DTYPE_BF16; }
+
+// Row strides of a [rows, cols] tensor: 0 = dense; false if rows would overlap or not be addressable.
+static bool row_stride_ok(size_t rows, size_t cols, size_t* stride) {
+  if (*stride == 0) *stride = cols;
+  return *stride >= cols && rows <= (SIZE_MAX >> 4) / *stride;
+}
+
+lcError_t lcLayerNormForward(const void* x, const void* gamma, const void* beta, void* out, float* mean, float* rstd,
+                             size_t rows, size_t cols, size_t x_stride, size_t out_stride, float eps,
+                             lcDataType dtype, lcDataType param_dtype, lcStream_t stream) {
+  if (!x || !out || rows == 0 || cols == 0 || !(eps >= 0.0f)) return LC_INVALID_VALUE;
+  if (!row_stride_ok(rows, cols, &x_stride) || !row_stride_ok(rows, cols, &out_stride)) return LC_INVALID_VALUE;
+  if (!float_type(dtype) || !float_type(param_dtype) || cols > (size_t)INT_MAX) return LC_NOT_SUPPORTED;
+  const LayerNormArgs a{x,    gamma,    beta,       out, mean,
+                        rstd, rows,     cols,       x_stride, out_stride,
+                        eps,  dtype == LC_DTYPE_BF16, param_dtype == LC_DTYPE_BF16};
+  LC_TRY(layer_norm_forward(a, static_cast<cudaStream_t>(stream)));
+  return LC_SUCCESS;
+}
+
+lcError_t lcLayerNormBackward(const void* dout, const void* x, const void* gamma, const float* mean,
+                              const float* rstd, void* dx, void* dgamma, void* dbeta, size_t rows, size_t cols,
+                              size_t dout_stride, size_t x_stride, size_t dx_stride, lcDataType dtype,
+                              lcDataType param_dtype, lcStream_t stream) {
+  if (!dout || !x || !mean || !rstd || (!dx && !dgamma && !dbeta) || rows == 0 || cols == 0) return LC_INVALID_VALUE;
+  if (!row_stride_ok(rows, cols, &dout_stride) || !row_stride_ok(rows, cols, &x_stride) ||
+      !row_stride_ok(rows, cols, &dx_stride))
+    return LC_INVALID_VALUE;
+  if (!float_type(dtype) || !float_type(param_dtype) || cols > (size_t)INT_MAX) return LC_NOT_SUPPORTED;
+  const LayerNormGradArgs a{dout, x,    gamma, mean,        rstd,     dx,        dgamma,
+                            dbeta, rows, cols,  dout_stride, x_stride, dx_stride, dtype == LC_DTYPE_BF16,
+                            param_dtype == LC_DTYPE_BF16};
+  LC_TRY(layer_norm_backward(a, static_cast<cudaStream_t>(stream)));
+  return LC_SUCCESS;
+}
+
+// Strides of a [batch, heads, len, dim] tensor, dense when all are 0; false when an offset would not
+// fit 60 bits.
+static bool head_strides(const lcHeadStrides& in, size_t batch, size_t heads, size_t len, size_t dim,
+                         HeadStrides* out) {
+  size_t total;
+  if (__builtin_mul_overflow(batch * heads, len, &total) || __builtin_mul_overflow(total, dim, &total) ||
+      total >> 58)
+    return false;  // (batch * heads fits 62 bits: each is an int)
+  lcHeadStrides s = in;
+  if (s.batch == 0 && s.head == 0 && s.token == 0) s = {heads * len * dim, len * dim, dim};
+  const size_t lim = size_t(1) << 58;
+  const auto fits = [&](size_t stride, size_t n) { return stride < lim && (stride == 0 || n <= lim / stride); };
+  if (!fits(s.batch, batch) || !fits(s.head, heads) || !fits(s.token, len)) return false;
+  *out = {static_cast<long long>(s.batch), static_cast<long long>(s.head), static_cast<long long>(s.token)};
+  return true;
+}
+
+// Whether no two elements of a written tensor share memory: with the axes sorted by stride, each one
+// steps over all that lies below it.
+static bool strides_disjoint(const HeadStrides& s, size_t batch, size_t heads, size_t len, size_t dim) {
+  long long stride[3] = {s.b, s.h, s.t};
+  size_t n[3] = {batch, heads, len};
+  for (int i = 0; i < 2; ++i)
+    for (int j = 0; j < 2 - i; ++j)
+      if (stride[j] > stride[j + 1]) {
+        std::swap(stride[j], stride[j + 1]);
+        std::swap(n[j], n[j + 1]);
+      }
+  long long span = static_cast<long long>(dim);
+  for (int i = 0; i < 3; ++i) {
+    if (n[i] == 1) continue;
+    if (stride[i] < span) return false;
+    span += stride[i] * static_cast<long long>(n[i] - 1);
+  }
+  return true;
+}
+
+// Checks a descriptor and fills everything but the tensors' pointers.
+static lcError_t cross_args(const lcCrossAttentionDesc* desc, CrossArgs* a) {
+  if (!desc) return LC_INVALID_VALUE;
+  const lcCrossAttentionDesc& d = *desc;
+  if (d.batch == 0 || d.q_heads == 0 || d.kv_heads == 0 || d.q_len == 0 || d.kv_len == 0 || d.head_dim == 0 ||
+      d.q_heads % d.kv_heads != 0)
+    return LC_INVALID_VALUE;
+  if (!(d.scale >= 0.0f) || std::isinf(d.scale)) return LC_INVALID_VALUE;
+  if (!float_type(d.dtype) || d.head_dim > 256) return LC_NOT_SUPPORTED;
+  const size_t lim = INT_MAX - 1024;  // room for an index to run past the end of a last tile
+  if (d.batch > lim || d.q_heads > lim || d.q_len > lim || d.kv_len > lim || d.kv_heads > lim || d.batch > lim / d.q_heads ||
+      d.q_heads / d.kv_heads > lim / d.q_len)
+    return LC_NOT_SUPPORTED;
+  if (!head_strides(d.q, d.batch, d.q_heads, d.q_len, d.head_dim, &a->qs) ||
+      !head_strides(d.k, d.batch, d.kv_heads, d.kv_len, d.head_dim, &a->ks) ||
+      !head_strides(d.v, d.batch, d.kv_heads, d.kv_len, d.head_dim, &a->vs) ||
+      !head_strides(d.out, d.batch, d.q_heads, d.q_len, d.head_dim, &a->os))
+    return LC_INVALID_VALUE;
+  if (!strides_disjoint(a->os, d.batch, d.q_heads, d.q_len, d.head_dim)) return LC_INVALID_VALUE;
+  a->q_lens = d.q_lens;
+  a->kv_lens = d.kv_lens;
+  a->key_mask = d.key_mask;
+  a->batch = static_cast<int>(d.batch);
+  a->hq = static_cast<int>(d.q_heads);
+  a->hk = static_cast<int>(d.kv_heads);
+  a->q_len = static_cast<int>(d.q_len);
+  a->kv_len = static_cast<int>(d.kv_len);
+  a->d = static_cast<int>(d.head_dim);
+  a->scale = d.scale == 0.0f ? 1.0f / sqrtf(static_cast<float>(d.head_dim)) : d.scale;
+  a->bf16 = d.dtype == LC_DTYPE_BF16;
+  return LC_SUCCESS;
+}
+
+lcError_t lcCrossAttentionForward(const lcCrossAttentionDesc* desc, const void* q, const void* k, const void* v,
+                                  void* out, float* lse, const lcAttentionIoPolicy* policy, lcStream_t stream) {
+  CrossArgs a{};
+  const lcError_t st = cross_args(desc, &a);
+  if (st != LC_SUCCESS) return st;
+  if (!q || !k || !v || !out) return LC_INVALID_VALUE;
+  lcAttentionIoPolicy pol;
+  if (policy) {
+    pol = *policy;
+  } else {
+    lcAttentionIoPolicyDefault(&pol);
+    pol.upload_q = pol.upload_k = pol.upload_v = pol.download_out = pol.synchronize = 0;
+  }
+  if (!neutral_postprocess(pol)) return LC_NOT_SUPPORTED;
+  // Host tensors are copied whole, so they are dense.
+  const auto dense = [](const lcHeadStrides& s) { return s.batch == 0 && s.head == 0 && s.token == 0; };
+  if ((pol.upload_q && !dense(desc->q)) || (pol.upload_k && !dense(desc->k)) || (pol.upload_v && !dense(desc->v)) ||
+      (pol.download_out && !dense(desc->out)))
+    return LC_NOT_SUPPORTED;
+  Io io(static_cast<cudaStream_t>(stream));
+  const size_t es = elem_size(desc->dtype);
+  const size_t q_rows = desc->batch * desc->q_heads * desc->q_len;
+  const size_t kv_bytes = desc->batch * desc->kv_heads * desc->kv_len * desc->head_dim * es;
+  const size_t q_bytes = q_rows * desc->head_dim * es;
+  const void* in[6] = {q, k, v, desc->q_lens, desc->kv_lens, desc->key_mask};
+  LC_TRY(io.in(q, q_bytes, pol.upload_q, &in[0]));
+  LC_TRY(io.in(k, kv_bytes, pol.upload_k, &in[1]));
+  LC_TRY(io.in(v, kv_bytes, pol.upload_v, &in[2]));
+  if (desc->q_lens) LC_TRY(io.in(desc->q_lens, desc->batch * sizeof(int32_t), pol.upload_q, &in[3]));
+  if (desc->kv_lens) LC_TRY(io.in(desc->kv_lens, desc->batch * sizeof(int32_t), pol.upload_k, &in[4]));
+  if (desc->key_mask) LC_TRY(io.in(desc->key_mask, desc->batch * desc->kv_len, pol.upload_k, &in[5]));
+  void *dout, *dlse = nullptr;
+  LC_TRY(io.out(out, q_bytes, pol.download_out, &dout));
+  if (lse) LC_TRY(io.out(lse, q_rows * 4, pol.download_out, &dlse));
+  if (pol.download_out && desc->q_lens) {
+    // Rows past q_lens keep what the caller's arrays hold, although the arrays come back whole.
+    LC_TRY(cudaMemcpyAsync(dout, out, q_bytes, cudaMemcpyHostToDevice, io.stream()));
+    if (lse) LC_TRY(cudaMemcpyAsync(dlse, lse, q_rows * 4, cudaMemcpyHostToDevice, io.stream()));
+  }
+  a.q = in[0];
+  a.k = in[1];
+  a.v = in[2];
+  a.q_lens = static_cast<const int*>(in[3]);
+  a.kv_lens = static_cast<const int*>(in[4]);
+  a.key_mask = static_cast<const unsigned char*>(in[5]);
+  a.out = dout;
+  a.lse = static_cast<float*>(dlse);
+  trace_op(kOpAttention, q_rows * desc->kv_len * desc->head_dim);
+  LC_TRY(cross_attention_forward(a, io.stream()));
+  if (lse && pol.download_out)
+    LC_TRY(cudaMemcpyAsync(lse, dlse, q_rows * 4, cudaMemcpyDeviceToHost, io.stream()));
+  LC_TRY(io.finish(out, dout, q_bytes, pol.download_out, pol.synchronize));
+  return check_error_word(pol.synchronize || pol.download_out);
+}
+
+lcError_t lcCrossAttentionBackward(const lcCrossAttentionDesc* desc, const void* dout, const void* q, const void* k,
+                                   const void* v, const void* out, const float* lse, void* dq, void* dk, void* dv,
+                                   lcStream_t stream) {
+  CrossGradArgs g{};
+  CrossArgs& a = g.f;
+  const lcError_t st = cross_args(desc, &a);
+  if (st != LC_SUCCESS) return st;
+  if (!dout || !q || !k || !v || !out || !lse || (!dq && !dk && !dv) || !dk != !dv) return LC_INVALID_VALUE;
+  if (dq && !strides_disjoint(a.qs, desc->batch, desc->q_heads, desc->q_len, desc->head_dim)) return LC_INVALID_VALUE;
+  g.kv_shared = desc->batch > 1 && a.ks.b == 0 && a.vs.b == 0;
+  const size_t kv_batch = g.kv_shared ? 1 : desc->batch;
+  if (dk && (!strides_disjoint(a.ks, kv_batch, desc->kv_heads, desc->kv_len, desc->head_dim) ||
+             !strides_disjoint(a.vs, kv_batch, desc->kv_heads, desc->kv_len, desc->head_dim)))
+    return LC_INVALID_VALUE;
+  a.q = q;
+  a.k = k;
+  a.v = v;
+  a.out = const_cast<void*>(out);
+  a.lse = const_cast<float*>(lse);
+  g.dout = dout;
+  g.dq = dq;
+  g.dk = dk;
+  g.dv = dv;
+  trace_op(kOpAttention, desc->batch * desc->q_heads * desc->q_len * desc->kv_len * desc->head_dim);
+  LC_TRY(cross_attention_backward(g, static_cast<cudaStream_t>(stream)));
   return LC_SUCCESS;
 }
 

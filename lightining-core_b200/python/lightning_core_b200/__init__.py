@@ -52,6 +52,18 @@ class Conv2dIoPolicy(C.Structure):
     _fields_ = [(n, C.c_int) for n in ("upload_x", "upload_w", "upload_bias", "download_out", "synchronize")]
 
 
+class HeadStrides(C.Structure):
+    """lcHeadStrides: elements from one batch entry, head and token to the next (all 0: dense)."""
+    _fields_ = [(n, C.c_size_t) for n in ("batch", "head", "token")]
+
+
+class CrossAttentionDesc(C.Structure):
+    """lcCrossAttentionDesc; :func:`cross_attention_desc` fills one."""
+    _fields_ = [(n, C.c_size_t) for n in ("batch", "q_heads", "kv_heads", "q_len", "kv_len", "head_dim")] + [
+        (n, HeadStrides) for n in ("q", "k", "v", "out")] + [
+        (n, C.c_void_p) for n in ("q_lens", "kv_lens", "key_mask")] + [("scale", C.c_float), ("dtype", C.c_int)]
+
+
 class RuntimeTraceEvent(C.Structure):
     _fields_ = [("type", C.c_int), ("status", C.c_int), ("timestamp_ns", C.c_uint64), ("size_bytes", C.c_size_t),
                 ("detail0", C.c_int), ("detail1", C.c_int)]
@@ -90,6 +102,10 @@ _SIGS = {
     "lcAttentionQkvProjForward": (_i, [_vp, _sz, _vp, _vp, _sz, _sz, _sz, C.POINTER(AttentionIoPolicy), _vp]),
     "lcVectorAdd": (_i, [_vp, _vp, _vp, _sz, _i, C.POINTER(VectorAddIoPolicy), _vp]),
     "lcLayerNorm": (_i, [_vp, _vp, _sz, _sz, _f, _vp]),
+    "lcLayerNormForward": (_i, [_vp] * 6 + [_sz] * 4 + [_f, _i, _i, _vp]),
+    "lcLayerNormBackward": (_i, [_vp] * 8 + [_sz] * 5 + [_i, _i, _vp]),
+    "lcCrossAttentionForward": (_i, [C.POINTER(CrossAttentionDesc)] + [_vp] * 5 + [C.POINTER(AttentionIoPolicy), _vp]),
+    "lcCrossAttentionBackward": (_i, [C.POINTER(CrossAttentionDesc)] + [_vp] * 10),
     "lcGetDeviceErrorWord": (_i, [C.POINTER(C.c_uint)]),
     "lcClearDeviceErrorWord": (_i, []),
     "lcRuntimeTraceSetEnabled": (None, [_i]),
@@ -485,6 +501,134 @@ def layer_norm(x, eps=1e-5):
     check(lib.lcLayerNorm(dx.ptr, dy.ptr, rows, cols, eps, None), "layer_norm")
     check(lib.lcDeviceSynchronize(), "sync")
     return dy.download(x.shape, np.float32)
+
+
+# ---- the cross-attention layer of an encoder-decoder -------------------------------------------
+def _typed(a, name, dtype):
+    """A contiguous host array of a tensor type: float32, or uint16 bf16 bits with dtype=BF16."""
+    if dtype not in (F32, BF16):
+        raise ValueError("dtype must be F32 or BF16")
+    a = np.ascontiguousarray(a) if dtype == BF16 else np.ascontiguousarray(a, dtype=np.float32)
+    if dtype == BF16 and a.dtype != np.uint16:
+        raise ValueError(f"{name} must hold bf16 bits (uint16) with dtype=BF16")
+    return a
+
+
+def _device(a):
+    return None if a is None else DeviceBuffer.from_array(a)
+
+
+def _ptr(buf):
+    return None if buf is None else buf.ptr
+
+
+def layer_norm_affine(x, gamma=None, beta=None, eps=1e-5, dtype: int = F32):
+    """Layer norm with weights over the last axis (lcLayerNormForward): host x (float32, or uint16 bf16
+    bits with dtype=BF16), float32 gamma / beta of the last axis' size (None: 1 / 0).
+    Returns (out, mean, rstd), the statistics float32 over the leading axes, for
+    :func:`layer_norm_backward`."""
+    x = _typed(x, "x", dtype)
+    if x.ndim < 1 or x.size == 0:
+        raise ValueError("x must have a last axis and elements")
+    cols = x.shape[-1]
+    rows = x.size // cols
+    w = [None if t is None else _f32(t, "weight").reshape(-1) for t in (gamma, beta)]
+    if any(t is not None and t.size != cols for t in w):
+        raise ValueError("gamma and beta must have the size of x's last axis")
+    dx, dg, db = _device(x), _device(w[0]), _device(w[1])
+    dy, stats = DeviceBuffer(x.nbytes), DeviceBuffer(8 * rows)
+    check(lib.lcLayerNormForward(dx.ptr, _ptr(dg), _ptr(db), dy.ptr, stats.value, stats.value + 4 * rows, rows, cols, 0,
+                                 0, eps, dtype, F32, None), "layer_norm_affine")
+    check(lib.lcDeviceSynchronize(), "sync")
+    mean, rstd = stats.download((2, rows), np.float32)
+    return dy.download(x.shape, x.dtype), mean.reshape(x.shape[:-1]), rstd.reshape(x.shape[:-1])
+
+
+def layer_norm_backward(dout, x, mean, rstd, gamma=None, dtype: int = F32):
+    """Gradients of :func:`layer_norm_affine` (lcLayerNormBackward): returns (dx, dgamma, dbeta), dx of
+    x's type, the weights' gradients float32."""
+    x, dout = _typed(x, "x", dtype), _typed(dout, "dout", dtype)
+    if x.ndim < 1 or x.size == 0 or dout.shape != x.shape:
+        raise ValueError("dout must have x's shape")
+    cols = x.shape[-1]
+    rows = x.size // cols
+    mean, rstd = (_f32(t, "statistics").reshape(-1) for t in (mean, rstd))
+    gamma = None if gamma is None else _f32(gamma, "gamma").reshape(-1)
+    if mean.size != rows or rstd.size != rows or (gamma is not None and gamma.size != cols):
+        raise ValueError("mean and rstd must have one value per row, gamma one per column")
+    dd, dx, dm, dr, dg = (_device(t) for t in (dout, x, mean, rstd, gamma))
+    gx, gw = DeviceBuffer(x.nbytes), DeviceBuffer(8 * cols)
+    check(lib.lcLayerNormBackward(dd.ptr, dx.ptr, _ptr(dg), dm.ptr, dr.ptr, gx.ptr, gw.value, gw.value + 4 * cols, rows,
+                                  cols, 0, 0, 0, dtype, F32, None), "layer_norm_backward")
+    check(lib.lcDeviceSynchronize(), "sync")
+    dgamma, dbeta = gw.download((2, cols), np.float32)
+    return gx.download(x.shape, x.dtype), dgamma, dbeta
+
+
+def cross_attention_desc(batch: int, q_heads: int, kv_heads: int, q_len: int, kv_len: int, head_dim: int,
+                         dtype: int = F32, q=(0, 0, 0), k=(0, 0, 0), v=(0, 0, 0), out=(0, 0, 0), q_lens=None,
+                         kv_lens=None, key_mask=None, scale: float = 0.0) -> CrossAttentionDesc:
+    """The descriptor of lcCrossAttentionForward / lcCrossAttentionBackward.  q, k, v, out: (batch, head,
+    token) strides in elements, (0, 0, 0) = dense [batch, heads, len, head_dim].  q_lens, kv_lens, key_mask:
+    addresses (device, or host where the call's policy uploads them) or None."""
+    return CrossAttentionDesc(batch, q_heads, kv_heads, q_len, kv_len, head_dim, tuple(q), tuple(k), tuple(v),
+                              tuple(out), q_lens, kv_lens, key_mask, scale, dtype)
+
+
+def _cross_shapes(q, k, v):
+    if q.ndim != 4 or k.ndim != 4 or v.shape != k.shape:
+        raise ValueError("q must be [batch, q_heads, q_len, head_dim], k and v [batch, kv_heads, kv_len, head_dim]")
+    b, hq, nq, d = q.shape
+    _, hk, nk, _ = k.shape
+    if k.shape[0] != b or k.shape[3] != d or hk == 0 or hq % hk:
+        raise ValueError("q, k and v must agree in batch and head_dim, and q_heads must be a multiple of kv_heads")
+    return b, hq, hk, nq, nk, d
+
+
+def _cross_masks(b, nk, q_lens, kv_lens, key_mask):
+    ql, kl = (None if t is None else np.ascontiguousarray(t, dtype=np.int32) for t in (q_lens, kv_lens))
+    if any(t is not None and t.shape != (b,) for t in (ql, kl)):
+        raise ValueError("q_lens and kv_lens must have one length per batch entry")
+    km = None if key_mask is None else np.ascontiguousarray(np.asarray(key_mask) != 0, dtype=np.uint8)
+    if km is not None and km.shape != (b, nk):
+        raise ValueError("key_mask must be [batch, kv_len]")
+    return ql, kl, km
+
+
+def cross_attention(q, k, v, kv_lens=None, key_mask=None, q_lens=None, scale: float = 0.0, dtype: int = F32):
+    """Attention of q [batch, q_heads, q_len, d] over k, v [batch, kv_heads, kv_len, d] (host arrays,
+    float32, or uint16 bf16 bits with dtype=BF16); q_heads a multiple of kv_heads.  Keys at or past
+    kv_lens, or with a 0 in key_mask [batch, kv_len], are masked; rows at or past q_lens stay 0.
+    scale 0 = 1/sqrt(d).  Returns (out, lse), the second for :func:`cross_attention_backward`."""
+    q, k, v = _typed(q, "q", dtype), _typed(k, "k", dtype), _typed(v, "v", dtype)
+    b, hq, hk, nq, nk, d = _cross_shapes(q, k, v)
+    ql, kl, km = _cross_masks(b, nk, q_lens, kv_lens, key_mask)
+    out, lse = np.zeros_like(q), np.zeros((b, hq, nq), np.float32)
+    desc = cross_attention_desc(b, hq, hk, nq, nk, d, dtype, q_lens=_vp(ql), kv_lens=_vp(kl), key_mask=_vp(km),
+                                scale=scale)
+    check(lib.lcCrossAttentionForward(desc, _vp(q), _vp(k), _vp(v), _vp(out), _vp(lse),
+                                      C.byref(default_attention_policy()), None), "cross_attention")
+    return out, lse
+
+
+def cross_attention_backward(dout, q, k, v, out, lse, kv_lens=None, key_mask=None, q_lens=None, scale: float = 0.0,
+                             dtype: int = F32):
+    """Gradients (dq, dk, dv) of :func:`cross_attention` from its inputs and results; rows of dq at or past
+    q_lens stay 0."""
+    dout, q, k, v, out = (_typed(t, n, dtype) for t, n in zip((dout, q, k, v, out), ("dout", "q", "k", "v", "out")))
+    b, hq, hk, nq, nk, d = _cross_shapes(q, k, v)
+    lse = _f32(lse, "lse")
+    if dout.shape != q.shape or out.shape != q.shape or lse.shape != (b, hq, nq):
+        raise ValueError("dout and out must have q's shape, lse [batch, q_heads, q_len]")
+    masks = [_device(t) for t in _cross_masks(b, nk, q_lens, kv_lens, key_mask)]
+    ins = [_device(t) for t in (dout, q, k, v, out, lse)]
+    grads = [DeviceBuffer.from_array(np.zeros_like(t)) for t in (q, k, v)]
+    desc = cross_attention_desc(b, hq, hk, nq, nk, d, dtype, q_lens=_ptr(masks[0]), kv_lens=_ptr(masks[1]),
+                                key_mask=_ptr(masks[2]), scale=scale)
+    check(lib.lcCrossAttentionBackward(desc, *[t.ptr for t in ins], *[t.ptr for t in grads], None),
+          "cross_attention_backward")
+    check(lib.lcDeviceSynchronize(), "sync")
+    return tuple(g.download(t.shape, t.dtype) for g, t in zip(grads, (q, k, v)))
 
 
 # ---- auto-tune cache ------------------------------------------------------------------------
