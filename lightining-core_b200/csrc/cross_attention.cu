@@ -531,7 +531,7 @@ cudaError_t fwd_simt(const CrossArgs& a, cudaStream_t s) {
   const long long blocks = (rows + TT - 1) / TT * a.batch * a.hk;
   if (blocks > 0x7fffffffLL) return cudaErrorNotSupported;
   CrossSplitWork w;
-  e = w.begin(a, blocks, TT, s);
+  e = w.begin(a, blocks, TT, 2, s);
   if (e != cudaSuccess) return e;
   const int vec = vec4(a.q, a.qs, a.d, sizeof(T)) && vec4(a.k, a.ks, a.d, sizeof(T)) && vec4(a.v, a.vs, a.d, sizeof(T));
   cross_fwd_simt_kernel<T, DP, TT>
@@ -614,13 +614,12 @@ cudaError_t bwd_any(const CrossGradArgs& g, cudaStream_t s) {
 }  // namespace
 
 // Splits a problem of `blocks` row tiles along its key tiles (of `tile` keys) when the blocks alone
-// leave SMs idle: enough parts for two blocks to an SM, at least one key tile each.
-cudaError_t CrossSplitWork::begin(const CrossArgs& a, long long blocks, int tile, cudaStream_t s) {
+// leave SMs idle: as many parts as fill `per_sm` blocks to an SM, at least one key tile each.
+cudaError_t CrossSplitWork::begin(const CrossArgs& a, long long blocks, int tile, int per_sm, cudaStream_t s) {
   DeviceCtx* ctx = device_ctx();
   if (!ctx) return cudaErrorNoDevice;
-  const long long tiles = (a.kv_len + tile - 1) / tile, want = 2LL * ctx->sm_count;
-  long long n = std::min<long long>({(want + blocks - 1) / blocks, tiles, 64});
-  if (blocks >= ctx->sm_count) n = 1;
+  const long long tiles = (a.kv_len + tile - 1) / tile, room = static_cast<long long>(per_sm) * ctx->sm_count;
+  const long long n = std::max(1LL, std::min<long long>({room / blocks, tiles, 64}));
   sp.splits = static_cast<int>(n);
   sp.rows = static_cast<long long>(a.batch) * a.hq * a.q_len;
   sp.o = nullptr;
@@ -650,6 +649,7 @@ cudaError_t CrossSplitWork::end(const CrossArgs& a, cudaError_t e, cudaStream_t 
 }
 
 cudaError_t cross_attention_forward(const CrossArgs& a, cudaStream_t s) {
+  if (cross_tc_supported(a)) return cross_forward_tc(a, s);
   return a.bf16 ? fwd_simt_any<__nv_bfloat16>(a, s) : fwd_simt_any<float>(a, s);
 }
 

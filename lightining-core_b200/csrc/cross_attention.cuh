@@ -23,8 +23,13 @@ struct CrossSplit {
 struct CrossSplitWork {
   CrossSplit sp{};
   void* ws = nullptr;
-  cudaError_t begin(const CrossArgs& a, long long blocks, int tile, cudaStream_t s);
+  cudaError_t begin(const CrossArgs& a, long long blocks, int tile, int per_sm, cudaStream_t s);
   cudaError_t end(const CrossArgs& a, cudaError_t launched, cudaStream_t s);
 };
+
+// bf16 on the tensor cores (cross_attention_sm100.cu): head_dim <= 128 and a multiple of 8, rows of 16-byte
+// alignment.
+bool cross_tc_supported(const CrossArgs& a);
+cudaError_t cross_forward_tc(const CrossArgs& a, cudaStream_t s);
 
 }  // namespace lcb
