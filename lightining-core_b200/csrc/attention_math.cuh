@@ -33,6 +33,11 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
   return d;
 }
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
 // 2^x for a pair of scores on the FMA pipes instead of MUFU: x = i + f with i = rint(x) (adding
 // and subtracting 1.5 * 2^23), f in [-0.5, 0.5]; 2^f by a degree-3 polynomial whose coefficients
 // are a weighted-least-squares minimax fit of 2^f on that interval (relative error 7.5e-5, far

@@ -192,6 +192,14 @@ __device__ __forceinline__ void tma_load_4d(void* smem_dst, const CUtensorMap* m
       : "memory");
 }
 
+// Untiled bulk load: `bytes` (a multiple of 16) from a 16-byte aligned address; counted on `bar`.
+__device__ __forceinline__ void bulk_load(void* smem_dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                   smem_u32(smem_dst)),
+               "l"(src), "r"(bytes), "r"(smem_u32(bar))
+               : "memory");
+}
+
 // Im2col-mode 4-D TMA load (tensor [n, h, w, c] fp32, coordinates {c, w, h, n} of the pixel box's
 // first pixel, plus the kernel-tap offsets {w, h}); completion counted on `bar`.  No multicast.
 __device__ __forceinline__ void tma_load_im2col_4d(void* smem_dst, const CUtensorMap* map, int c, int w, int h, int n,

@@ -311,11 +311,12 @@ __global__ void __launch_bounds__(256) cross_combine_kernel(CrossArgs a, CrossSp
 }
 
 // ---- backward -------------------------------------------------------------------------------
-// Row terms: D = dout . out, and the row's log-sum-exp in the log2 domain.  Rows that are not
-// computed or see no key get (+infinity, 0): every weight exp2(s - inf) is 0.  One warp to a row;
-// rows of the workspace are padded to whole tiles of 128 tokens.
+// Row terms, negated so that they are addends: -D with D = dout . out, and minus the row's
+// log-sum-exp in the log2 domain.  Rows that are not computed or see no key get -infinity and 0:
+// every weight exp2(s - inf) is 0.  One warp to a row; rows of the workspace are padded to whole
+// tiles of 128 tokens.
 template <typename T>
-__global__ void __launch_bounds__(256) cross_row_terms_kernel(CrossGradArgs g, float* lse2, float* delta, int q_pad,
+__global__ void __launch_bounds__(256) cross_row_terms_kernel(CrossGradArgs g, float* neg_lse2, float* neg_d, int q_pad,
                                                               long long rows) {
   const CrossArgs& a = g.f;
   const long long row = static_cast<long long>(blockIdx.x) * 8 + (threadIdx.x >> 5);
@@ -324,11 +325,11 @@ __global__ void __launch_bounds__(256) cross_row_terms_kernel(CrossGradArgs g, f
   const int t = static_cast<int>(row % q_pad);
   const long long bh = row / q_pad;
   const int h = static_cast<int>(bh % a.hq), b = static_cast<int>(bh / a.hq);
-  float sum = 0.0f, lse = INFINITY;
+  float sum = 0.0f, lse = -INFINITY;
   if (t < cross_len(a.q_lens, b, a.q_len)) {
     const float x = a.lse[bh * a.q_len + t];
     if (x != -INFINITY) {
-      lse = x * kLog2e;
+      lse = -x * kLog2e;
       const long long at = b * a.os.b + h * a.os.h + t * a.os.t;
       const T *o = static_cast<const T*>(a.out) + at, *d = static_cast<const T*>(g.dout) + at;
       for (int c = lane; c < a.d; c += 32) sum = fmaf(to_f(o[c]), to_f(d[c]), sum);
@@ -336,15 +337,15 @@ __global__ void __launch_bounds__(256) cross_row_terms_kernel(CrossGradArgs g, f
   }
   sum = lanes_sum<32>(sum);
   if (lane == 0) {
-    lse2[row] = lse;
-    delta[row] = sum;
+    neg_lse2[row] = lse;
+    neg_d[row] = -sum;
   }
 }
 
 // dq of one tile of TT rows of a (batch, key head) pair.
 template <typename T, int DP, int TT>
-__global__ void __launch_bounds__(Tile<DP, TT>::NT) cross_dq_simt_kernel(CrossGradArgs g, const float* lse2,
-                                                                         const float* delta, int q_pad, int vec) {
+__global__ void __launch_bounds__(Tile<DP, TT>::NT) cross_dq_simt_kernel(CrossGradArgs g, const float* neg_lse2,
+                                                                         const float* neg_d, int q_pad, int vec) {
   using L = Tile<DP, TT>;
   const CrossArgs& a = g.f;
   extern __shared__ __align__(16) float smem[];
@@ -377,8 +378,8 @@ __global__ void __launch_bounds__(Tile<DP, TT>::NT) cross_dq_simt_kernel(CrossGr
     int h, t;
     const bool in = at(rg + i * L::GL, h, t);
     const long long w = (static_cast<long long>(b) * a.hq + h) * q_pad + t;
-    lse[i] = in ? lse2[w] : INFINITY;
-    del[i] = in ? delta[w] : 0.0f;
+    lse[i] = in ? neg_lse2[w] : -INFINITY;
+    del[i] = in ? neg_d[w] : 0.0f;
     f[i] = a.scale;
 #pragma unroll
     for (int c = 0; c < L::CPT; ++c) o[i][c] = 0.0f;
@@ -401,8 +402,8 @@ __global__ void __launch_bounds__(Tile<DP, TT>::NT) cross_dq_simt_kernel(CrossGr
     for (int i = 0; i < 4; ++i)
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const float p = exp2f(fmaf(s[i][j], sc, -lse[i]));
-        P[(rg + i * L::GL) * L::LP + cg + j * L::GL] = seen[cg + j * L::GL] ? p * (dp[i][j] - del[i]) : 0.0f;
+        const float p = exp2f(fmaf(s[i][j], sc, lse[i]));
+        P[(rg + i * L::GL) * L::LP + cg + j * L::GL] = seen[cg + j * L::GL] ? p * (dp[i][j] + del[i]) : 0.0f;
       }
     __syncthreads();
     acc_tile<DP, TT>(P, K, rg, cg, o);
@@ -413,8 +414,8 @@ __global__ void __launch_bounds__(Tile<DP, TT>::NT) cross_dq_simt_kernel(CrossGr
 // dk and / or dv of one tile of TT keys of a (batch, key head) pair: the group's rows, one tile after
 // the other, and every batch entry in turn when k and v are shared by them.
 template <typename T, int DP, int TT, bool DK, bool DV>
-__global__ void __launch_bounds__(Tile<DP, TT>::NT) cross_dkv_simt_kernel(CrossGradArgs g, const float* lse2,
-                                                                          const float* delta, int q_pad, int vec) {
+__global__ void __launch_bounds__(Tile<DP, TT>::NT) cross_dkv_simt_kernel(CrossGradArgs g, const float* neg_lse2,
+                                                                          const float* neg_d, int q_pad, int vec) {
   using L = Tile<DP, TT>;
   const CrossArgs& a = g.f;
   extern __shared__ __align__(16) float smem[];
@@ -467,8 +468,8 @@ __global__ void __launch_bounds__(Tile<DP, TT>::NT) cross_dkv_simt_kernel(CrossG
         int h, t;
         const bool in = at(tid, h, t);
         const long long w = (static_cast<long long>(b) * a.hq + h) * q_pad + t;
-        row_lse[tid] = in ? lse2[w] : INFINITY;
-        row_del[tid] = in ? delta[w] : 0.0f;
+        row_lse[tid] = in ? neg_lse2[w] : -INFINITY;
+        row_del[tid] = in ? neg_d[w] : 0.0f;
       }
       __syncthreads();
       float s[4][4], dp[4][4];
@@ -477,7 +478,7 @@ __global__ void __launch_bounds__(Tile<DP, TT>::NT) cross_dkv_simt_kernel(CrossG
       for (int i = 0; i < 4; ++i)
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-          s[i][j] = seen[rg + i * L::GL] ? exp2f(fmaf(s[i][j], sc, -row_lse[cg + j * L::GL])) : 0.0f;
+          s[i][j] = seen[rg + i * L::GL] ? exp2f(fmaf(s[i][j], sc, row_lse[cg + j * L::GL])) : 0.0f;
       if constexpr (DV) {
 #pragma unroll
         for (int i = 0; i < 4; ++i)
@@ -493,7 +494,7 @@ __global__ void __launch_bounds__(Tile<DP, TT>::NT) cross_dkv_simt_kernel(CrossG
         for (int i = 0; i < 4; ++i)
 #pragma unroll
           for (int j = 0; j < 4; ++j)
-            P[(rg + i * L::GL) * L::LP + cg + j * L::GL] = s[i][j] * (dp[i][j] - row_del[cg + j * L::GL]);
+            P[(rg + i * L::GL) * L::LP + cg + j * L::GL] = s[i][j] * (dp[i][j] + row_del[cg + j * L::GL]);
         __syncthreads();
         acc_tile<DP, TT>(P, Q, rg, cg, dk);
       }
@@ -547,7 +548,7 @@ cudaError_t fwd_simt_any(const CrossArgs& a, cudaStream_t s) {
 }
 
 template <typename T, int DP, int TT>
-cudaError_t bwd_simt(const CrossGradArgs& g, const float* lse2, const float* delta, int q_pad, cudaStream_t s) {
+cudaError_t bwd_simt(const CrossGradArgs& g, const float* neg_lse2, const float* neg_d, int q_pad, cudaStream_t s) {
   using L = Tile<DP, TT>;
   const CrossArgs& a = g.f;
   constexpr size_t SMEM = (4 * L::ROWS + L::SQ) * sizeof(float);
@@ -561,7 +562,7 @@ cudaError_t bwd_simt(const CrossGradArgs& g, const float* lse2, const float* del
     const long long rows = static_cast<long long>(a.hq / a.hk) * a.q_len;
     const long long blocks = (rows + TT - 1) / TT * a.batch * a.hk;
     if (blocks > 0x7fffffffLL) return cudaErrorNotSupported;
-    cross_dq_simt_kernel<T, DP, TT><<<static_cast<unsigned>(blocks), L::NT, SMEM, s>>>(g, lse2, delta, q_pad, vec);
+    cross_dq_simt_kernel<T, DP, TT><<<static_cast<unsigned>(blocks), L::NT, SMEM, s>>>(g, neg_lse2, neg_d, q_pad, vec);
     if ((e = cudaGetLastError()) != cudaSuccess) return e;
   }
   if (g.dk) {
@@ -573,15 +574,15 @@ cudaError_t bwd_simt(const CrossGradArgs& g, const float* lse2, const float* del
       static std::atomic<unsigned long long> attr{0};
       e = allow_smem(attr, cross_dkv_simt_kernel<T, DP, TT, true, true>, SMEM);
       if (e != cudaSuccess) return e;
-      cross_dkv_simt_kernel<T, DP, TT, true, true><<<n, L::NT, SMEM, s>>>(g, lse2, delta, q_pad, vec);
+      cross_dkv_simt_kernel<T, DP, TT, true, true><<<n, L::NT, SMEM, s>>>(g, neg_lse2, neg_d, q_pad, vec);
     } else {
       // Two passes: both gradients' sums of 256 columns would not fit the registers.
       static std::atomic<unsigned long long> attr_k{0}, attr_v{0};
       if ((e = allow_smem(attr_k, cross_dkv_simt_kernel<T, DP, TT, true, false>, SMEM)) != cudaSuccess) return e;
       if ((e = allow_smem(attr_v, cross_dkv_simt_kernel<T, DP, TT, false, true>, SMEM)) != cudaSuccess) return e;
-      cross_dkv_simt_kernel<T, DP, TT, true, false><<<n, L::NT, SMEM, s>>>(g, lse2, delta, q_pad, vec);
+      cross_dkv_simt_kernel<T, DP, TT, true, false><<<n, L::NT, SMEM, s>>>(g, neg_lse2, neg_d, q_pad, vec);
       if ((e = cudaGetLastError()) != cudaSuccess) return e;
-      cross_dkv_simt_kernel<T, DP, TT, false, true><<<n, L::NT, SMEM, s>>>(g, lse2, delta, q_pad, vec);
+      cross_dkv_simt_kernel<T, DP, TT, false, true><<<n, L::NT, SMEM, s>>>(g, neg_lse2, neg_d, q_pad, vec);
     }
     e = cudaGetLastError();
   }
@@ -600,13 +601,15 @@ cudaError_t bwd_any(const CrossGradArgs& g, cudaStream_t s) {
   void* ws = nullptr;
   cudaError_t e = workspace_alloc(ctx, &ws, static_cast<size_t>(rows) * 2 * sizeof(float), s);
   if (e != cudaSuccess) return e;
-  float *lse2 = static_cast<float*>(ws), *delta = lse2 + rows;
-  cross_row_terms_kernel<T><<<static_cast<unsigned>(blocks), 256, 0, s>>>(g, lse2, delta, q_pad, rows);
+  float *neg_lse2 = static_cast<float*>(ws), *neg_d = neg_lse2 + rows;
+  cross_row_terms_kernel<T><<<static_cast<unsigned>(blocks), 256, 0, s>>>(g, neg_lse2, neg_d, q_pad, rows);
   e = cudaGetLastError();
-  if (e == cudaSuccess)
-    e = a.d <= 64    ? bwd_simt<T, 64, 64>(g, lse2, delta, q_pad, s)
-        : a.d <= 128 ? bwd_simt<T, 128, 64>(g, lse2, delta, q_pad, s)
-                     : bwd_simt<T, 256, 32>(g, lse2, delta, q_pad, s);
+  if (e == cudaSuccess && cross_grad_tc_supported(g))
+    e = cross_backward_tc(g, neg_lse2, neg_d, q_pad, s);
+  else if (e == cudaSuccess)
+    e = a.d <= 64    ? bwd_simt<T, 64, 64>(g, neg_lse2, neg_d, q_pad, s)
+        : a.d <= 128 ? bwd_simt<T, 128, 64>(g, neg_lse2, neg_d, q_pad, s)
+                     : bwd_simt<T, 256, 32>(g, neg_lse2, neg_d, q_pad, s);
   const cudaError_t f = workspace_free(ws, s);
   return e != cudaSuccess ? e : f;
 }

@@ -31,5 +31,9 @@ struct CrossSplitWork {
 // alignment.
 bool cross_tc_supported(const CrossArgs& a);
 cudaError_t cross_forward_tc(const CrossArgs& a, cudaStream_t s);
+// neg_lse2, neg_d: the row terms, [batch * q_heads][q_pad], q_pad whole tiles of 128 tokens.
+bool cross_grad_tc_supported(const CrossGradArgs& g);
+cudaError_t cross_backward_tc(const CrossGradArgs& g, const float* neg_lse2, const float* neg_d, int q_pad,
+                              cudaStream_t s);
 
 }  // namespace lcb
