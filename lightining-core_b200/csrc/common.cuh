@@ -76,6 +76,7 @@ enum : unsigned {
   kErrCrossLoadWait = 0x301,
   kErrCrossMmaWait = 0x302,
   kErrCrossSoftmaxWait = 0x303,
+  kErrNormLoadWait = 0x401,
 };
 
 __device__ __forceinline__ uint64_t globaltimer_ns() {
