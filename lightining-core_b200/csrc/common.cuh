@@ -201,6 +201,13 @@ __device__ __forceinline__ void bulk_load(void* smem_dst, const void* src, uint3
                : "memory");
 }
 
+// 16 bytes global -> shared without registers; zeros when `ok` is false (nothing is read then).
+__device__ __forceinline__ void cp_async16(void* smem_dst, const void* src, bool ok) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(smem_dst)), "l"(src), "r"(ok ? 16 : 0)
+               : "memory");
+}
+__device__ __forceinline__ void cp_async_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+
 // Im2col-mode 4-D TMA load (tensor [n, h, w, c] fp32, coordinates {c, w, h, n} of the pixel box's
 // first pixel, plus the kernel-tap offsets {w, h}); completion counted on `bar`.  No multicast.
 __device__ __forceinline__ void tma_load_im2col_4d(void* smem_dst, const CUtensorMap* map, int c, int w, int h, int n,
@@ -241,6 +248,13 @@ __device__ __forceinline__ void tma_store_3d(const CUtensorMap* map, const void*
   asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.bulk_group [%0, {%2, %3, %4}], [%1];" ::"l"(
                    reinterpret_cast<uint64_t>(map)),
                "r"(smem_u32(smem_src)), "r"(c0), "r"(c1), "r"(c2)
+               : "memory");
+}
+__device__ __forceinline__ void tma_store_4d(const CUtensorMap* map, const void* smem_src, int c0, int c1, int c2,
+                                             int c3) {
+  asm volatile("cp.async.bulk.tensor.4d.global.shared::cta.bulk_group [%0, {%2, %3, %4, %5}], [%1];" ::"l"(
+                   reinterpret_cast<uint64_t>(map)),
+               "r"(smem_u32(smem_src)), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
                : "memory");
 }
 // 2-D TMA store shared -> global (bulk async-group completion); out-of-range rows/columns are
@@ -365,6 +379,18 @@ __device__ __forceinline__ bool warp_wait_poll(uint64_t* bar, uint32_t parity, v
   }
   return __all_sync(0xffffffffu, ok);
 }
+// The same for a barrier that is mostly complete already when it is asked for: the first poll decides for
+// the whole warp without a vote (it is one instruction on one address), and the bounded loop is kept out of
+// the way.
+static __device__ __noinline__ bool warp_wait_slow(uint64_t* bar, uint32_t parity, volatile int* abort_flag,
+                                                   unsigned* err_word, unsigned code) {
+  return warp_wait_poll(bar, parity, abort_flag, err_word, code);
+}
+__device__ __forceinline__ bool warp_wait_ready(uint64_t* bar, uint32_t parity, volatile int* abort_flag,
+                                                unsigned* err_word, unsigned code) {
+  if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
+  return warp_wait_slow(bar, parity, abort_flag, err_word, code);
+}
 // The same MMAs and commit issued from a converged warp: every lane executes the call and one
 // lane, chosen by elect.sync inside the asm, issues.  Keeping the whole warp on the issue path lets
 // the operands stay warp-uniform; a loop run by lane 0 alone issues slower.
@@ -404,6 +430,73 @@ __device__ __forceinline__ void umma_commit_w(uint64_t* bar) {
   asm volatile(
       "{\n .reg .pred e;\n elect.sync _|e, 0xffffffff;\n"
       " @e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}\n" ::"r"(smem_u32(bar))
+      : "memory");
+}
+// Four MMAs of one 64-deep K chunk from a converged warp, one elect.sync for all of them: the issue
+// slots between two MMAs are what a warp beside busy ones pays for.  Both operands K-major with 128-byte
+// swizzle: 16 values = 32 bytes = 2 descriptor units on per step.
+__device__ __forceinline__ void umma_f16_ss4_w(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                               uint32_t accumulate) {
+  asm volatile(
+      "{\n .reg .pred p, t, e;\n .reg .b64 a1, b1, a2, b2, a3, b3;\n"
+      " setp.ne.b32 p, %4, 0;\n setp.eq.b32 t, 0, 0;\n"
+      " add.s64 a1, %1, 2;\n add.s64 b1, %2, 2;\n add.s64 a2, %1, 4;\n add.s64 b2, %2, 4;\n"
+      " add.s64 a3, %1, 6;\n add.s64 b3, %2, 6;\n"
+      " elect.sync _|e, 0xffffffff;\n"
+      " @e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n"
+      " @e tcgen05.mma.cta_group::1.kind::f16 [%0], a1, b1, %3, t;\n"
+      " @e tcgen05.mma.cta_group::1.kind::f16 [%0], a2, b2, %3, t;\n"
+      " @e tcgen05.mma.cta_group::1.kind::f16 [%0], a3, b3, %3, t;\n}\n" ::"r"(d_tmem),
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// The same with B MN-major (16 rows of 128 bytes = 128 descriptor units on).
+__device__ __forceinline__ void umma_f16_ss4n_w(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                                uint32_t accumulate) {
+  asm volatile(
+      "{\n .reg .pred p, t, e;\n .reg .b64 a1, b1, a2, b2, a3, b3;\n"
+      " setp.ne.b32 p, %4, 0;\n setp.eq.b32 t, 0, 0;\n"
+      " add.s64 a1, %1, 2;\n add.s64 b1, %2, 128;\n add.s64 a2, %1, 4;\n add.s64 b2, %2, 256;\n"
+      " add.s64 a3, %1, 6;\n add.s64 b3, %2, 384;\n"
+      " elect.sync _|e, 0xffffffff;\n"
+      " @e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n"
+      " @e tcgen05.mma.cta_group::1.kind::f16 [%0], a1, b1, %3, t;\n"
+      " @e tcgen05.mma.cta_group::1.kind::f16 [%0], a2, b2, %3, t;\n"
+      " @e tcgen05.mma.cta_group::1.kind::f16 [%0], a3, b3, %3, t;\n}\n" ::"r"(d_tmem),
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// The same with A in TMEM (16 bf16 values = 8 columns on per step) and B MN-major (16 rows of 128 bytes
+// = 128 descriptor units on).
+__device__ __forceinline__ void umma_f16_ts4_w(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc,
+                                               uint32_t accumulate) {
+  asm volatile(
+      "{\n .reg .pred p, t, e;\n .reg .b32 a1, a2, a3;\n .reg .b64 b1, b2, b3;\n"
+      " setp.ne.b32 p, %4, 0;\n setp.eq.b32 t, 0, 0;\n"
+      " add.s32 a1, %1, 8;\n add.s32 a2, %1, 16;\n add.s32 a3, %1, 24;\n"
+      " add.s64 b1, %2, 128;\n add.s64 b2, %2, 256;\n add.s64 b3, %2, 384;\n"
+      " elect.sync _|e, 0xffffffff;\n"
+      " @e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n"
+      " @e tcgen05.mma.cta_group::1.kind::f16 [%0], [a1], b1, %3, t;\n"
+      " @e tcgen05.mma.cta_group::1.kind::f16 [%0], [a2], b2, %3, t;\n"
+      " @e tcgen05.mma.cta_group::1.kind::f16 [%0], [a3], b3, %3, t;\n}\n" ::"r"(d_tmem),
+      "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// A in TMEM, B K-major.
+__device__ __forceinline__ void umma_f16_ts4k_w(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc,
+                                               uint32_t accumulate) {
+  asm volatile(
+      "{\n .reg .pred p, t, e;\n .reg .b32 a1, a2, a3;\n .reg .b64 b1, b2, b3;\n"
+      " setp.ne.b32 p, %4, 0;\n setp.eq.b32 t, 0, 0;\n"
+      " add.s32 a1, %1, 8;\n add.s32 a2, %1, 16;\n add.s32 a3, %1, 24;\n"
+      " add.s64 b1, %2, 2;\n add.s64 b2, %2, 4;\n add.s64 b3, %2, 6;\n"
+      " elect.sync _|e, 0xffffffff;\n"
+      " @e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n"
+      " @e tcgen05.mma.cta_group::1.kind::f16 [%0], [a1], b1, %3, t;\n"
+      " @e tcgen05.mma.cta_group::1.kind::f16 [%0], [a2], b2, %3, t;\n"
+      " @e tcgen05.mma.cta_group::1.kind::f16 [%0], [a3], b3, %3, t;\n}\n" ::"r"(d_tmem),
+      "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
       : "memory");
 }
 // Warp-uniform bounded wait: lane 0 waits, the result is broadcast.

@@ -6,6 +6,7 @@
 #include <math.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "attention_math.cuh"
 #include "common.cuh"
@@ -46,28 +47,29 @@ __device__ __forceinline__ void drain_bar(uint64_t* bar, uint32_t ph) {
 // Zeroes the rows of a staged tile for which keep(row) is false (one warp).  Swizzling permutes
 // inside a row only.  The matrix unit multiplies a masked row by a weight of 0, which would keep a
 // NaN or an infinity that memory holds there.
-template <int NCH, class Keep>
+template <int NCH, int ROWS, class Keep>
 __device__ __forceinline__ void scrub_rows(uint8_t* tile, Keep keep) {
   const int lane = threadIdx.x & 31;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
+  for (int i = 0; i < ROWS / 32; ++i) {
     const int row = i * 32 + lane;
     if (!keep(row))
       for (int c = 0; c < NCH; ++c)
 #pragma unroll
         for (int e = 0; e < 8; ++e)
-          *reinterpret_cast<uint4*>(tile + c * CH + row * 128 + e * 16) = make_uint4(0, 0, 0, 0);
+          *reinterpret_cast<uint4*>(tile + (c * ROWS + row) * 128 + e * 16) = make_uint4(0, 0, 0, 0);
   }
   fence_proxy_async_smem();
   __syncwarp();
 }
 
-// Visible keys of the tile at kv0 as four words of 32 (bit e of word i: key kv0 + 32 i + e).  `byte`
-// are this lane's four mask bytes (loaded early); without a mask only the end of the keys counts.
+// Whether this lane's keys of the tile at kv0 (kv0 + 32 i + lane) are visible; a ballot of byte[i]
+// gives every lane the word of those 32 keys.  Loaded ahead of the wait for the scores.
+template <int N>
 __device__ __forceinline__ void load_mask_bytes(const unsigned char* mask, int kv0, int kv_end, int lane,
-                                                unsigned char (&byte)[4]) {
+                                                unsigned char (&byte)[N]) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
+  for (int i = 0; i < N; ++i) {
     const int k = kv0 + i * 32 + lane;
     byte[i] = k < kv_end && (!mask || mask[k]);
   }
@@ -221,19 +223,15 @@ __global__ void __launch_bounds__(Fwd<D>::THREADS, 1)
       const uint64_t qd = smem_desc_sw128(smem_u32(sQ(h)), 16, 1024);
       const uint64_t kd = smem_desc_sw128(smem_u32(sK(j % NS)), 16, 1024);
 #pragma unroll
-      for (int kk = 0; kk < D / 16; ++kk) {
-        const uint32_t o16 = ((kk >> 2) * CH + (kk & 3) * 32) >> 4;
-        umma_f16_ss_w(tmem + h * 128, qd + o16, kd + o16, IDESC_S, kk > 0 ? 1u : 0u);
-      }
+      for (int c = 0; c < D / 64; ++c)
+        umma_f16_ss4_w(tmem + h * 128, qd + (c * CH >> 4), kd + (c * CH >> 4), IDESC_S, c > 0 ? 1u : 0u);
       issued = true;
       umma_commit_w(&st->s_full[h]);
     };
     const auto issue_pv = [&](int h, int j) {
       const uint64_t vd = smem_desc_sw128(smem_u32(sV(j % NS)), CH, 1024);
-#pragma unroll
-      for (int kk = 0; kk < TILE / 16; ++kk)
-        umma_f16_ts_w(tmem + 256 + h * 128, tmem + h * 128 + kk * 8, vd + (kk * 2048 >> 4), IDESC_O,
-                      (j > 0 || kk > 0) ? 1u : 0u);
+      umma_f16_ts4_w(tmem + 256 + h * 128, tmem + h * 128, vd, IDESC_O, j > 0 ? 1u : 0u);
+      umma_f16_ts4_w(tmem + 256 + h * 128, tmem + h * 128 + 32, vd + (4 * 2048 >> 4), IDESC_O, 1u);
       umma_commit_w(&st->o_done[h]);
     };
     if (n > 0) {
@@ -252,7 +250,7 @@ __global__ void __launch_bounds__(Fwd<D>::THREADS, 1)
       if (!(ok = wait(&st->v_full[s], (j / NS) & 1))) break;
       // Masked rows of V: keys past kv_end that memory holds (TMA zero-fills past kv_len), and holes.
       if (mask || (kv0 + TILE > kv_end && kv_end < a.kv_len))
-        scrub_rows<F::NCH>(sV(s), [&](int r) { return kv0 + r < kv_end && (!mask || mask[kv0 + r]); });
+        scrub_rows<F::NCH, TILE>(sV(s), [&](int r) { return kv0 + r < kv_end && (!mask || mask[kv0 + r]); });
       for (int h = 0; h < 2 && ok; ++h) {
         if (!act[h]) continue;
         // p_full[h] next completes for P_h(j+1), which needs S_h(j+1), issued after this wait.
@@ -436,122 +434,162 @@ __global__ void __launch_bounds__(Fwd<D>::THREADS, 1)
   }
 }
 
-// ---- backward: dk and dv ------------------------------------------------------------------------
-// One block per SM owns a tile of 128 keys of a (batch, key head) pair and walks the tiles of 128
-// queries of the group's heads ("items"; of every batch entry in turn when k and v are shared by
-// them).  Keys are the rows: S^T = K Q^T and dP^T = V dout^T arrive with a key per TMEM lane, so
-// P^T and dS^T go straight back to TMEM as the A operands of dV += P^T dout and dK += dS^T Q, whose B
-// operands are the same dout and Q tiles read MN-major.  Nothing is transposed or passed through
-// shared memory, and both gradients accumulate in TMEM: no atomics, one order of summation.
-//   warp 0      TMA: K and V once; Q, dout and the row terms of each item into NS stages
-//   warp 1      MMA, in the order S(0) dP(0) | dV(i) S(i+1) dK(i) dP(i+1): while the other warps form
-//               dS(i) the products dV(i) and S(i+1) run, while they form P(i+1) dK(i) and dP(i+1) do
-//   warps 2..9  P and dS: a thread owns a key (lane) and half of the item's queries
-// TMEM columns: S^T / P^T 0 (P of query half h over the first 32 columns of that half's scores),
-// dP^T / dS^T 128 (likewise), dV 256, dK 256 + D.
-template <int D>
-struct Dkv {
+// ---- backward -----------------------------------------------------------------------------------
+// One kernel walks both ways over the score matrix.  A job keeps 128 rows of one side and streams tiles of
+// 64 rows of the other ("items"):
+//   KV    rows are keys (X1 = K, X2 = V), items are queries of the group's heads, and of every batch
+//         entry in turn when k and v are shared by them (Y1 = Q, Y2 = dout): writes dk and dv
+//   else  rows are queries as in the forward pass (X1 = Q, X2 = dout), items are keys (Y1 = K, Y2 = V):
+//         writes dq
+// With S = X1 Y1^T, P = exp(S - lse), dP = X2 Y2^T, dS = P (dP - D), the sums over the items are
+// A1 += P Y2 (dv) and A2 += dS Y1 (dk or dq), both kept in TMEM.  P and dS come out with a row per TMEM
+// lane and go to shared memory as the A operands; Y1 and Y2 are read as they lie, MN-major: nothing is
+// transposed.  Forming S and dP once for each side costs two products, 7 instead of 5; taking dq from the
+// walk that yields dk and dv would need atomics, whose order changes the result, or fp32 partial rows of
+// every key tile in memory.
+// What bounds it is keeping three things busy at once that depend on each other: the tensor pipe (64-row
+// items: 650 cycles at head_dim 64, 1120 at 128), MUFU (512 cycles) and the issue slots of the warps that
+// form P and dS; a wait and a commit cost the issuing warp some 100 cycles each.  Hence
+//   * X1 and X2 in TMEM as A operands: an N = 64 product then takes 36 cycles a step instead of 53 (its
+//     operands in shared memory are what binds it), and shared memory holds more items
+//   * P and dS in shared memory, so the score columns are free as soon as they have been read, and the next
+//     item's products run while this one's weights are formed
+//   * two groups of eight warps that take the items in turn
+//   * three issuing warps, for S, dP and the sums, which order each other by barriers only
+//   * resident blocks that go from job to job: four more warps load the next job's rows and store
+//     the last one's sums meanwhile (two sets of TMEM columns where they fit)
+// Before: blocks of one job each with one chain of products took 271 (head_dim 64) and 150 us (128) for dk and
+// dv at [16, 16, 512 x 2048 ragged, 64] and [4, 16/4, 1024 x 2048 ragged, 128], tensor pipe 27% and 52% active.
+constexpr int QT = 64;         // rows of an item
+constexpr int QCH = QT * 128;  // one [64 rows x 64 bf16] box
+template <int D, bool KV>
+struct Grad {
   static constexpr int NCH = D / 64;
-  static constexpr int BYTES = NCH * CH;
-  static constexpr int NS = D == 64 ? 4 : 2;
-  static constexpr int STAGE = 2 * BYTES;   // Q, dout
-  static constexpr int STAGE_OFF = 2 * BYTES;
-  static constexpr int TERM_OFF = STAGE_OFF + NS * STAGE;  // [NS][2][128] floats
-  static constexpr int TAIL_OFF = TERM_OFF + NS * 1024;
-  static constexpr int THREADS = 320;
+  static constexpr int BYTES = NCH * QCH;    // a Y tile
+  static constexpr int STAGE = 2 * BYTES;
+  static constexpr bool X_SMEM = KV && D == 128;     // rows in shared memory, the TMEM columns are taken
+  static constexpr int NS = D == 64 ? 8 : 4;
+  static constexpr int NX = D == 64 ? 2 : 1;         // sets of rows
+  static constexpr int NA = D == 64 && !KV ? 2 : 1;  // sets of sums
+  static constexpr int X_OFF = NS * STAGE;           // [2][128 x D] bf16
+  static constexpr int TERM_OFF = X_OFF + (X_SMEM ? 2 * NCH * CH : 0);  // [NS][2][64] floats (KV)
+  // Boxes of [128 rows x 64 bf16]: next rows on their way to TMEM, and sums on their way to memory (as many
+  // as fit), a quarter to each of the four warps that move rows.
+  static constexpr int IN_OFF = TERM_OFF + (KV ? NS * 512 : 0);
+  static constexpr int OUT_OFF = IN_OFF + (X_SMEM ? 0 : 2 * NCH * CH);
+  static constexpr int OUTS = X_SMEM ? 1 : (KV ? 2 : 1) * NCH;
+  static constexpr int TAIL_OFF = OUT_OFF + OUTS * CH;
+  static constexpr int THREADS = 24 * 32;
+  // TMEM columns: rows, S, dP, P and dS of the two groups, sums.
+  static constexpr uint32_t X = 0, XW = X_SMEM ? 0 : D, S = NX * XW, DP = S + 64, P = DP + 64, DS = P + (KV ? 64 : 0),
+                            A = DS + 64, AW = KV ? 2 * D : D;
+  static_assert(A + NA * AW <= 512, "TMEM");
   struct Tail {
-    uint64_t kv_full;
-    uint64_t q_full[NS], g_full[NS], free_[NS];
-    uint64_t s_full, dp_full, p_full, ds_full, done;
-    uint64_t drain;
+    uint64_t full[NS], free_[NS];
+    uint64_t x_full[NX], done[NA], sums_free[NA], in_full, in_free;
+    uint64_t s_full[2], dp_full[2], p_full[2], ds_full[2], used[2];  // by group
+    uint64_t s_read, dp_read;
+    uint64_t drain[3];
     uint32_t tmem_base;
     int abort_flag;
   };
-  static constexpr size_t SMEM = 1024 + TAIL_OFF + sizeof(Tail);
+  static constexpr size_t SMEM = TAIL_OFF + sizeof(Tail);
+  static_assert(SMEM <= 227 * 1024, "shared memory");
 };
 
 struct GradParams {
   CrossGradArgs g;
   const float *neg_lse2, *neg_d;
   int q_pad;
-  int q_head, q_batch, g_head, g_batch, k_head, k_batch, v_head, v_batch;  // 1: the map has that axis
+  int y1_head, y1_batch, y2_head, y2_batch;  // 1: the map of the streamed tensor has that axis
+  int x1_head, x1_batch, x2_head, x2_batch;  // KV: the same of k and v, and of their gradients
+  int jobs, tiles;                           // tiles of rows of a (batch, key head) pair
   float scale_log2;
   unsigned* err;
 };
 
-// The items of a key tile, in order: batch entries that see a key of it, heads of the group, tiles of
-// their queries.
-struct Items {
-  const CrossArgs& a;
-  int k0, b_hi, group;
-  int b, g, qt, q_end, kv_end;  // the current item, and its batch entry's lengths
-  __device__ Items(const CrossArgs& a_, int k0_, int b_lo, int b_hi_)
-      : a(a_), k0(k0_), b_hi(b_hi_), group(a_.hq / a_.hk), b(b_lo), g(0), qt(0), q_end(0), kv_end(0) {
-    settle();
+// A job's rows.  Its items are, in order: the batch entries [b, b_hi) with span() > 0, `heads` heads each, tiles
+// of 64 rows up to span().
+template <bool KV>
+struct Job {
+  int b, hk, r0, b_hi, group, heads;
+  __device__ Job(const GradParams& p, int job) {
+    const CrossArgs& a = p.g.f;
+    const int pair = job / p.tiles;
+    b = pair / a.hk;
+    hk = pair % a.hk;
+    r0 = (job % p.tiles) * TILE;
+    b_hi = KV && p.g.kv_shared ? a.batch : b + 1;
+    group = a.hq / a.hk;
+    heads = KV ? group : 1;
   }
-  // Moves to the first batch entry from b on that has an item; b == b_hi: none left.
-  __device__ void settle() {
-    for (; b < b_hi; ++b) {
-      q_end = cross_len(a.q_lens, b, a.q_len);
-      kv_end = cross_len(a.kv_lens, b, a.kv_len);
-      if (k0 < kv_end && q_end > 0) return;
-    }
+  // Rows of batch entry yb to walk (0: none), for KV the queries if the tile has a key to see, else the keys if
+  // the tile has a query to compute: its first row's token is one, or another head starts in it.
+  __device__ int span(const CrossArgs& a, int yb) const {
+    const int q_end = cross_len(a.q_lens, yb, a.q_len), kv_end = cross_len(a.kv_lens, yb, a.kv_len);
+    if (KV) return r0 < kv_end ? q_end : 0;
+    const int t = r0 % a.q_len;
+    return q_end > 0 && (t < q_end || r0 + a.q_len - t < min(r0 + TILE, group * a.q_len)) ? kv_end : 0;
   }
-  __device__ bool valid() const { return b < b_hi; }
-  __device__ void next() {
-    if ((qt + 1) * TILE < q_end) {
-      ++qt;
-      return;
-    }
-    qt = 0;
-    if (++g < group) return;
-    g = 0;
-    ++b;
-    settle();
+  __device__ int count(const CrossArgs& a) const {
+    int n = 0;
+    for (int yb = b; yb < b_hi; ++yb) n += heads * ((span(a, yb) + QT - 1) / QT);
+    return n;
   }
 };
 
-template <int D>
-__global__ void __launch_bounds__(Dkv<D>::THREADS, 1)
-    cross_dkv_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_g,
-                        const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
-                        const GradParams p) {
-  using L = Dkv<D>;
-  constexpr int NS = L::NS;
-  extern __shared__ __align__(16) uint8_t smem_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+template <int D, bool KV>
+__global__ void __launch_bounds__(Grad<D, KV>::THREADS, 1)
+    cross_grad_tc_kernel(const __grid_constant__ CUtensorMap map_y1, const __grid_constant__ CUtensorMap map_y2,
+                         const __grid_constant__ CUtensorMap map_x1, const __grid_constant__ CUtensorMap map_x2,
+                         const __grid_constant__ CUtensorMap map_dk, const __grid_constant__ CUtensorMap map_dv,
+                         const GradParams p) {
+  using L = Grad<D, KV>;
+  constexpr int NS = L::NS, NX = L::NX, NA = L::NA;
+  extern __shared__ __align__(1024) uint8_t smem[];
+  if ((smem_u32(smem) & 1023u) != 0) {  // the 128-byte swizzle atoms need 1 KB alignment
+    if (threadIdx.x == 0) atomicCAS(p.err, 0u, static_cast<unsigned>(kErrCrossLoadWait) | 0x1000u);
+    return;
+  }
   typename L::Tail* st = reinterpret_cast<typename L::Tail*>(smem + L::TAIL_OFF);
-  uint8_t *sK = smem, *sV = smem + L::BYTES;
-  const auto sQ = [&](int s) { return smem + L::STAGE_OFF + s * L::STAGE; };
-  const auto sG = [&](int s) { return smem + L::STAGE_OFF + s * L::STAGE + L::BYTES; };
-  const auto terms = [&](int s) { return reinterpret_cast<float*>(smem + L::TERM_OFF + s * 1024); };
+  const auto sY1 = [&](int s) { return smem + s * L::STAGE; };
+  const auto sY2 = [&](int s) { return smem + s * L::STAGE + L::BYTES; };
+  const auto terms = [&](int s) { return reinterpret_cast<float*>(smem + L::TERM_OFF + s * 512); };
   const CrossArgs& a = p.g.f;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int key_tiles = (a.kv_len + TILE - 1) / TILE;
-  const int bh = blockIdx.x / key_tiles, b0 = bh / a.hk, hk = bh % a.hk;
-  const int k0 = (blockIdx.x % key_tiles) * TILE;
-  const int b_hi = p.g.kv_shared ? a.batch : b0 + 1;
-  const int group = a.hq / a.hk;
 
   if (threadIdx.x == 0) {
-    mbar_init(&st->kv_full, 1);
     for (int s = 0; s < NS; ++s) {
-      mbar_init(&st->q_full[s], 1);
-      mbar_init(&st->g_full[s], 1);
+      mbar_init(&st->full[s], 1);
       mbar_init(&st->free_[s], 1);
     }
-    mbar_init(&st->s_full, 1);
-    mbar_init(&st->dp_full, 1);
-    mbar_init(&st->p_full, 8);
-    mbar_init(&st->ds_full, 8);
-    mbar_init(&st->done, 1);
-    mbar_init(&st->drain, 1);
+    for (int x = 0; x < NX; ++x) mbar_init(&st->x_full[x], L::X_SMEM ? 1 : 4);
+    mbar_init(&st->in_full, 1);
+    mbar_init(&st->in_free, 4);
+    for (int x = 0; x < NA; ++x) {
+      mbar_init(&st->done[x], 1);
+      mbar_init(&st->sums_free[x], 4);
+    }
+    for (int c = 0; c < 2; ++c) {
+      mbar_init(&st->s_full[c], 1);
+      mbar_init(&st->dp_full[c], 1);
+      mbar_init(&st->p_full[c], 8);
+      mbar_init(&st->ds_full[c], 8);
+      mbar_init(&st->used[c], 1);
+    }
+    for (int c = 0; c < 3; ++c) mbar_init(&st->drain[c], 1);
+    mbar_init(&st->s_read, 8);
+    mbar_init(&st->dp_read, 8);
     st->abort_flag = 0;
     fence_barrier_init();
-    tma_prefetch_desc(&map_q);
-    tma_prefetch_desc(&map_g);
-    tma_prefetch_desc(&map_k);
-    tma_prefetch_desc(&map_v);
+    tma_prefetch_desc(&map_y1);
+    tma_prefetch_desc(&map_y2);
+    if (KV) {
+      tma_prefetch_desc(&map_x1);
+      tma_prefetch_desc(&map_x2);
+      tma_prefetch_desc(&map_dk);
+      tma_prefetch_desc(&map_dv);
+    }
   }
   if (warp == 0) {
     tmem_alloc(&st->tmem_base, 512);
@@ -562,513 +600,461 @@ __global__ void __launch_bounds__(Dkv<D>::THREADS, 1)
   tc_fence_after();
   const uint32_t tmem = st->tmem_base;
   volatile int* abort_flag = &st->abort_flag;
-  Items it(a, k0, b0, b_hi);
-  const bool any = it.valid();
+  const int grid = static_cast<int>(gridDim.x);
+  // Every role counts the items it has passed (i) and the jobs that have some (x); item i belongs to group
+  // i & 1 and stage i % NS, job x to columns x % NX and x % NA.  Each barrier's next completion needs
+  // what its waiters do after this one, so no parity wait is ambiguous.
 
   if (warp == 0) {
     // ------------------------------------------------------------ TMA producer
-    if (lane == 0 && any) {
-      bool ok = true;
-      int q_issued = 0, g_issued = 0;
-      mbar_arrive_expect_tx(&st->kv_full, 2 * L::BYTES);
-      load_tile(sK, &map_k, L::NCH, k0, p.k_head ? hk : 0, p.k_batch ? b0 : 0, &st->kv_full);
-      load_tile(sV, &map_v, L::NCH, k0, p.v_head ? hk : 0, p.v_batch ? b0 : 0, &st->kv_full);
-      for (int i = 0; it.valid(); it.next(), ++i) {
-        const int s = i % NS;
-        // free_[s] next completes for the item loaded here, so the parity wait is unambiguous.
-        if (i >= NS && !mbar_wait_bounded(&st->free_[s], (i / NS - 1) & 1, abort_flag, p.err, kErrCrossLoadWait)) {
-          ok = false;
-          break;
-        }
-        const int h = hk * group + it.g;
-        const long long term = (static_cast<long long>(it.b) * a.hq + h) * p.q_pad + it.qt * TILE;
-        mbar_arrive_expect_tx(&st->q_full[s], L::BYTES + 512);
-        load_tile(sQ(s), &map_q, L::NCH, it.qt * TILE, p.q_head ? h : 0, p.q_batch ? it.b : 0, &st->q_full[s]);
-        bulk_load(terms(s), p.neg_lse2 + term, 512, &st->q_full[s]);
-        ++q_issued;
-        mbar_arrive_expect_tx(&st->g_full[s], L::BYTES + 512);
-        load_tile(sG(s), &map_g, L::NCH, it.qt * TILE, p.g_head ? h : 0, p.g_batch ? it.b : 0, &st->g_full[s]);
-        bulk_load(terms(s) + 128, p.neg_d + term, 512, &st->g_full[s]);
-        ++g_issued;
-      }
-      if (!ok) {
-        drain_bar(&st->kv_full, 0);
-        for (int i = max(0, q_issued - NS); i < q_issued; ++i) drain_bar(&st->q_full[i % NS], (i / NS) & 1);
-        for (int i = max(0, g_issued - NS); i < g_issued; ++i) drain_bar(&st->g_full[i % NS], (i / NS) & 1);
-      }
-    }
-  } else if (warp == 1) {
-    // ------------------------------------------------------------ MMA issuer (whole warp)
-    constexpr uint32_t IDESC_S = idesc_bf16_f32(TILE, TILE, 0, 0);
-    constexpr uint32_t IDESC_G = idesc_bf16_f32(TILE, D, 0, 1);  // A in TMEM, B MN-major
-    bool ok = true, issued = false;
-    const auto wait = [&](uint64_t* bar, uint32_t ph) {
-      return warp_wait_poll(bar, ph, abort_flag, p.err, kErrCrossMmaWait);
-    };
-    // [128 keys x 128 queries] = A (keys) B^T (queries), both K-major, into column `col`.
-    const auto scores = [&](uint32_t col, const uint8_t* keys, const uint8_t* queries, uint64_t* bar) {
-      const uint64_t ad = smem_desc_sw128(smem_u32(keys), 16, 1024), bd = smem_desc_sw128(smem_u32(queries), 16, 1024);
-#pragma unroll
-      for (int kk = 0; kk < D / 16; ++kk) {
-        const uint32_t o16 = ((kk >> 2) * CH + (kk & 3) * 32) >> 4;
-        umma_f16_ss_w(tmem + col, ad + o16, bd + o16, IDESC_S, kk > 0 ? 1u : 0u);
-      }
-      issued = true;
-      umma_commit_w(bar);
-    };
-    // [128 keys x D] (+)= A (weights in TMEM at `col`) B (the item's rows, MN-major).
-    const auto grads = [&](uint32_t dst, uint32_t col, const uint8_t* queries, bool first) {
-      const uint64_t bd = smem_desc_sw128(smem_u32(queries), CH, 1024);
-#pragma unroll
-      for (int kk = 0; kk < TILE / 16; ++kk)
-        umma_f16_ts_w(tmem + dst, tmem + col + (kk >> 2) * 64 + (kk & 3) * 8, bd + (kk * 2048 >> 4), IDESC_G,
-                      (first && kk == 0) ? 0u : 1u);
-    };
-    // Rows past q_lens that memory holds are zeroed: they would enter both gradients' sums.
-    const auto ready = [&](uint64_t* bar, int i, uint8_t* tile, const Items& x) {
-      if (!wait(bar, (i / NS) & 1)) return false;
-      if (x.qt * TILE + TILE > x.q_end && x.q_end < a.q_len)
-        scrub_rows<L::NCH>(tile, [&](int r) { return x.qt * TILE + r < x.q_end; });
-      tc_fence_after();
-      return true;
-    };
-    if (any) {
-      ok = wait(&st->kv_full, 0) && ready(&st->q_full[0], 0, sQ(0), it);
-      if (ok) scores(0, sK, sQ(0), &st->s_full);
-      if (ok) ok = ready(&st->g_full[0], 0, sG(0), it);
-      if (ok) scores(128, sV, sG(0), &st->dp_full);
-      for (int i = 0; ok; ++i) {
-        const int s = i % NS, sn = (i + 1) % NS;
-        Items nx = it;
-        nx.next();
-        const bool more = nx.valid();
-        // p_full next completes for P(i+1), which needs S(i+1), issued after this wait.
-        if (!(ok = wait(&st->p_full, i & 1))) break;
-        tc_fence_after();
-        grads(256, 0, sG(s), i == 0);
-        if (more) {
-          if (!(ok = ready(&st->q_full[sn], i + 1, sQ(sn), nx))) break;
-          scores(0, sK, sQ(sn), &st->s_full);
-        }
-        // ds_full next completes for dS(i+1), which needs dP(i+1), issued after this wait.
-        if (!(ok = wait(&st->ds_full, i & 1))) break;
-        tc_fence_after();
-        grads(256 + D, 128, sQ(s), i == 0);
-        if (!more) {
-          umma_commit_w(&st->done);
-          break;
-        }
-        umma_commit_w(&st->free_[s]);
-        if (!(ok = ready(&st->g_full[sn], i + 1, sG(sn), nx))) break;
-        scores(128, sV, sG(sn), &st->dp_full);
-        it.next();
-      }
-    }
-    if (!ok && issued) {
-      umma_commit_w(&st->drain);
-      drain_bar(&st->drain, 0);
-    }
-  } else {
-    // ------------------------------------------------------------ P and dS
-    const int half = warp >= 6 ? 1 : 0, quarter = warp & 3;
-    const int row = quarter * 32 + lane, key = k0 + row;
-    const uint32_t lane_base = static_cast<uint32_t>(quarter * 32) << 16;
-    const uint32_t s_tmem = tmem + lane_base + half * 64, dp_tmem = s_tmem + 128;
-    bool ok = true, vis = false, ever = false;
-    int vis_b = -1;
-    const uint64_t sc2 = pk2(p.scale_log2, p.scale_log2);
-    for (int i = 0; it.valid(); it.next(), ++i) {
-      const int s = i % NS;
-      if (it.b != vis_b) {
-        vis_b = it.b;
-        vis = key < it.kv_end && (!a.key_mask || a.key_mask[static_cast<long long>(it.b) * a.kv_len + key]);
-        ever |= vis;
-      }
-      // The stage is refilled only after dS(i) of these very warps.
-      if (!(ok = warp_wait_poll(&st->q_full[s], (i / NS) & 1, abort_flag, p.err, kErrCrossSoftmaxWait) &&
-                 warp_wait_poll(&st->s_full, i & 1, abort_flag, p.err, kErrCrossSoftmaxWait)))
-        break;
-      tc_fence_after();
-      const float4* nl = reinterpret_cast<const float4*>(terms(s) + half * 64);
-      uint64_t pr[32];  // this key's weights of 64 queries
-#pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        uint32_t r[32], w[16];
-        tmem_ld32(s_tmem + c * 32, r);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const float4 t = nl[c * 8 + e];
-          float x0, x1, x2, x3;
-          unpk2(fma2(pk2(__uint_as_float(r[4 * e]), __uint_as_float(r[4 * e + 1])), sc2, pk2(t.x, t.y)), x0, x1);
-          unpk2(fma2(pk2(__uint_as_float(r[4 * e + 2]), __uint_as_float(r[4 * e + 3])), sc2, pk2(t.z, t.w)), x2, x3);
-          x0 = fast_exp2(x0);
-          x1 = fast_exp2(x1);
-          x2 = fast_exp2(x2);
-          x3 = fast_exp2(x3);
-          pr[c * 16 + 2 * e] = vis ? pk2(x0, x1) : 0;
-          pr[c * 16 + 2 * e + 1] = vis ? pk2(x2, x3) : 0;
-          w[2 * e] = vis ? pack_bf16x2(x0, x1) : 0u;
-          w[2 * e + 1] = vis ? pack_bf16x2(x2, x3) : 0u;
-        }
-        tmem_st16(s_tmem + c * 16, w);
-      }
-      tmem_wait_st();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&st->p_full);
-      if (!(ok = warp_wait_poll(&st->g_full[s], (i / NS) & 1, abort_flag, p.err, kErrCrossSoftmaxWait) &&
-                 warp_wait_poll(&st->dp_full, i & 1, abort_flag, p.err, kErrCrossSoftmaxWait)))
-        break;
-      tc_fence_after();
-      const float4* nd = reinterpret_cast<const float4*>(terms(s) + 128 + half * 64);
-#pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        uint32_t r[32], w[16];
-        tmem_ld32(dp_tmem + c * 32, r);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const float4 t = nd[c * 8 + e];
-          float x0, x1, x2, x3;
-          unpk2(mul2(pr[c * 16 + 2 * e], add2(pk2(__uint_as_float(r[4 * e]), __uint_as_float(r[4 * e + 1])), pk2(t.x, t.y))),
-                x0, x1);
-          unpk2(mul2(pr[c * 16 + 2 * e + 1],
-                     add2(pk2(__uint_as_float(r[4 * e + 2]), __uint_as_float(r[4 * e + 3])), pk2(t.z, t.w))),
-                x2, x3);
-          w[2 * e] = vis ? pack_bf16x2(x0, x1) : 0u;  // (a masked value may hold a NaN)
-          w[2 * e + 1] = vis ? pack_bf16x2(x2, x3) : 0u;
-        }
-        tmem_st16(dp_tmem + c * 16, w);
-      }
-      tmem_wait_st();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&st->ds_full);
-    }
-    if (ok && any) ok = warp_wait_poll(&st->done, 0, abort_flag, p.err, kErrCrossSoftmaxWait);
-    if (ok) {
-      tc_fence_after();
-      // Warps 2..5 store dv, 6..9 dk; a masked key's gradient is 0 whatever its row holds.
-      const HeadStrides& gs = half ? a.ks : a.vs;
-      const float f = half ? a.scale : 1.0f;
-      __nv_bfloat16* out =
-          static_cast<__nv_bfloat16*>(half ? p.g.dk : p.g.dv) + b0 * gs.b + hk * gs.h + static_cast<long long>(key) * gs.t;
-      const bool store = key < a.kv_len;
-#pragma unroll
-      for (int c = 0; c < D; c += 32) {
-        uint32_t o[32];
-        tmem_ld32(tmem + lane_base + 256 + half * D + c, o);
-        if (store) {
-#pragma unroll
-          for (int e = 0; e < 32; e += 8)
-            if (c + e < a.d) {
-              uint32_t w[4];
-#pragma unroll
-              for (int q = 0; q < 4; ++q)
-                w[q] = ever ? pack_bf16x2(__uint_as_float(o[e + 2 * q]) * f, __uint_as_float(o[e + 2 * q + 1]) * f) : 0u;
-              *reinterpret_cast<uint4*>(out + c + e) = make_uint4(w[0], w[1], w[2], w[3]);
-            }
-        }
-        __syncwarp();
-      }
-    }
-  }
-  tc_fence_before();
-  __syncthreads();
-  if (warp == 0) {
-    tc_fence_after();
-    tmem_dealloc(tmem, 512);
-  }
-}
-
-// ---- backward: dq -------------------------------------------------------------------------------
-// One block per SM owns a tile of 128 rows of a (batch, key head) pair (rows as in the forward pass) and
-// walks the key tiles: S = Q K^T and dP = dout V^T again, dS back to TMEM as the A operand of
-// dQ += dS K (K read MN-major).  Forming S and dP a second time costs two products, 7 instead of 5 in
-// the whole backward pass; adding dQ tiles from the kernel above would need either atomics, whose order
-// changes the result, or fp32 partial rows of every key tile in memory.
-//   warp 0      TMA: K_j and V_j into rings
-//   warp 1      MMA: S(0) dP(0) | S(j+1) dQ(j) dP(j+1): S alternates between two TMEM buffers, so it
-//               runs ahead while dS(j) is formed; masked rows of K_j are zeroed here
-//   warps 2..9  the Q and dout rows into shared memory, then dS: a thread owns a row and half the keys
-// TMEM columns: S 0 and 128, dP / dS 256, dQ 384.
-template <int D>
-struct Dq {
-  static constexpr int NCH = D / 64;
-  static constexpr int BYTES = NCH * CH;
-  static constexpr int NK = D == 64 ? 4 : 3;  // K stages: S(j+1) is issued while K_j serves dQ(j)
-  static constexpr int NV = D == 64 ? 4 : 2;
-  static constexpr int K_OFF = 2 * BYTES;  // after Q and dout
-  static constexpr int V_OFF = K_OFF + NK * BYTES;
-  static constexpr int TAIL_OFF = V_OFF + NV * BYTES;
-  static constexpr int THREADS = 320;
-  struct Tail {
-    uint64_t rows_full;  // 8 warp arrivals
-    uint64_t k_full[NK], k_free[NK], v_full[NV], v_free[NV];
-    uint64_t s_full[2], dp_full, ds_full, done;
-    uint64_t drain;
-    uint32_t tmem_base;
-    int abort_flag;
-  };
-  static constexpr size_t SMEM = 1024 + TAIL_OFF + sizeof(Tail);
-};
-
-template <int D>
-__global__ void __launch_bounds__(Dq<D>::THREADS, 1)
-    cross_dq_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
-                       const GradParams p) {
-  using L = Dq<D>;
-  constexpr int NK = L::NK, NV = L::NV;
-  extern __shared__ __align__(16) uint8_t smem_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  typename L::Tail* st = reinterpret_cast<typename L::Tail*>(smem + L::TAIL_OFF);
-  uint8_t *sQ = smem, *sG = smem + L::BYTES;
-  const auto sK = [&](int s) { return smem + L::K_OFF + s * L::BYTES; };
-  const auto sV = [&](int s) { return smem + L::V_OFF + s * L::BYTES; };
-  const CrossArgs& a = p.g.f;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int group = a.hq / a.hk, rows = group * a.q_len;
-  const int row_tiles = (rows + TILE - 1) / TILE;
-  const int bh = blockIdx.x / row_tiles, b = bh / a.hk, hk = bh % a.hk;
-  const int r0 = (blockIdx.x % row_tiles) * TILE;
-  const int q_end = cross_len(a.q_lens, b, a.q_len), kv_end = cross_len(a.kv_lens, b, a.kv_len);
-  const int n = (kv_end + TILE - 1) / TILE;
-  {
-    const int t = r0 % a.q_len;  // no row of the tile is computed: leave (uniform over the block)
-    if (q_end == 0 || (t >= q_end && r0 + a.q_len - t >= min(r0 + TILE, rows))) return;
-  }
-  const unsigned char* mask = a.key_mask ? a.key_mask + static_cast<long long>(b) * a.kv_len : nullptr;
-
-  if (threadIdx.x == 0) {
-    mbar_init(&st->rows_full, 8);
-    for (int s = 0; s < NK; ++s) {
-      mbar_init(&st->k_full[s], 1);
-      mbar_init(&st->k_free[s], 1);
-    }
-    for (int s = 0; s < NV; ++s) {
-      mbar_init(&st->v_full[s], 1);
-      mbar_init(&st->v_free[s], 1);
-    }
-    mbar_init(&st->s_full[0], 1);
-    mbar_init(&st->s_full[1], 1);
-    mbar_init(&st->dp_full, 1);
-    mbar_init(&st->ds_full, 8);
-    mbar_init(&st->done, 1);
-    mbar_init(&st->drain, 1);
-    st->abort_flag = 0;
-    fence_barrier_init();
-    tma_prefetch_desc(&map_k);
-    tma_prefetch_desc(&map_v);
-  }
-  if (warp == 0) {
-    tmem_alloc(&st->tmem_base, 512);
-    tmem_relinquish();
-  }
-  tc_fence_before();
-  __syncthreads();
-  tc_fence_after();
-  const uint32_t tmem = st->tmem_base;
-  volatile int* abort_flag = &st->abort_flag;
-
-  if (warp == 0) {
-    // ------------------------------------------------------------ TMA producer
-    if (lane == 0) {
-      bool ok = true;
-      int k_issued = 0, v_issued = 0;
-      for (int j = 0; j < n; ++j) {
-        const int s = j % NK, sv = j % NV;
-        if (j >= NK && !mbar_wait_bounded(&st->k_free[s], (j / NK - 1) & 1, abort_flag, p.err, kErrCrossLoadWait)) {
-          ok = false;
-          break;
-        }
-        mbar_arrive_expect_tx(&st->k_full[s], L::BYTES);
-        load_tile(sK(s), &map_k, L::NCH, j * TILE, p.k_head ? hk : 0, p.k_batch ? b : 0, &st->k_full[s]);
-        ++k_issued;
-        if (j >= NV && !mbar_wait_bounded(&st->v_free[sv], (j / NV - 1) & 1, abort_flag, p.err, kErrCrossLoadWait)) {
-          ok = false;
-          break;
-        }
-        mbar_arrive_expect_tx(&st->v_full[sv], L::BYTES);
-        load_tile(sV(sv), &map_v, L::NCH, j * TILE, p.v_head ? hk : 0, p.v_batch ? b : 0, &st->v_full[sv]);
-        ++v_issued;
-      }
-      if (!ok) {
-        for (int j = max(0, k_issued - NK); j < k_issued; ++j) drain_bar(&st->k_full[j % NK], (j / NK) & 1);
-        for (int j = max(0, v_issued - NV); j < v_issued; ++j) drain_bar(&st->v_full[j % NV], (j / NV) & 1);
-      }
-    }
-  } else if (warp == 1) {
-    // ------------------------------------------------------------ MMA issuer (whole warp)
-    constexpr uint32_t IDESC_S = idesc_bf16_f32(TILE, TILE, 0, 0);
-    constexpr uint32_t IDESC_G = idesc_bf16_f32(TILE, D, 0, 1);
-    bool ok = true, issued = false;
-    const auto wait = [&](uint64_t* bar, uint32_t ph) {
-      return warp_wait_poll(bar, ph, abort_flag, p.err, kErrCrossMmaWait);
-    };
-    const auto scores = [&](uint32_t col, const uint8_t* queries, const uint8_t* keys, uint64_t* bar) {
-      const uint64_t ad = smem_desc_sw128(smem_u32(queries), 16, 1024), bd = smem_desc_sw128(smem_u32(keys), 16, 1024);
-#pragma unroll
-      for (int kk = 0; kk < D / 16; ++kk) {
-        const uint32_t o16 = ((kk >> 2) * CH + (kk & 3) * 32) >> 4;
-        umma_f16_ss_w(tmem + col, ad + o16, bd + o16, IDESC_S, kk > 0 ? 1u : 0u);
-      }
-      issued = true;
-      umma_commit_w(bar);
-    };
-    const auto k_ready = [&](int j) {
-      if (!wait(&st->k_full[j % NK], (j / NK) & 1)) return false;
-      const int kv0 = j * TILE;
-      // Masked rows of K enter the sum of dQ with a weight of 0: zeroed, in case they hold a NaN.
-      if (mask || (kv0 + TILE > kv_end && kv_end < a.kv_len))
-        scrub_rows<L::NCH>(sK(j % NK), [&](int r) { return kv0 + r < kv_end && (!mask || mask[kv0 + r]); });
-      tc_fence_after();
-      return true;
-    };
-    if (n > 0) {
-      ok = wait(&st->rows_full, 0) && k_ready(0);
-      if (ok) scores(0, sQ, sK(0), &st->s_full[0]);
-      if (ok) ok = wait(&st->v_full[0], 0);
-      if (ok) {
-        tc_fence_after();
-        scores(256, sG, sV(0), &st->dp_full);
-        if (NV < n) umma_commit_w(&st->v_free[0]);
-      }
-    }
-    for (int j = 0; j < n && ok; ++j) {
-      if (j + 1 < n) {
-        // Buffer (j+1)&1 held S(j-1), which those warps had read before ds_full(j-1).
-        if (!(ok = k_ready(j + 1))) break;
-        scores(((j + 1) & 1) * 128, sQ, sK((j + 1) % NK), &st->s_full[(j + 1) & 1]);
-      }
-      // ds_full next completes for dS(j+1), which needs dP(j+1), issued after this wait.
-      if (!(ok = wait(&st->ds_full, j & 1))) break;
-      tc_fence_after();
-      const uint64_t bd = smem_desc_sw128(smem_u32(sK(j % NK)), CH, 1024);
-#pragma unroll
-      for (int kk = 0; kk < TILE / 16; ++kk)
-        umma_f16_ts_w(tmem + 384, tmem + 256 + (kk >> 2) * 64 + (kk & 3) * 8, bd + (kk * 2048 >> 4), IDESC_G,
-                      (j == 0 && kk == 0) ? 0u : 1u);
-      if (j + 1 == n) {
-        umma_commit_w(&st->done);
-        break;
-      }
-      if (j + NK < n) umma_commit_w(&st->k_free[j % NK]);
-      if (!(ok = wait(&st->v_full[(j + 1) % NV], ((j + 1) / NV) & 1))) break;
-      tc_fence_after();
-      scores(256, sG, sV((j + 1) % NV), &st->dp_full);
-      if (j + 1 + NV < n) umma_commit_w(&st->v_free[(j + 1) % NV]);
-    }
-    if (!ok && issued) {
-      umma_commit_w(&st->drain);
-      drain_bar(&st->drain, 0);
-    }
-  } else {
-    // ------------------------------------------------------------ rows: Q and dout in, dS, dq out
-    const int half = warp >= 6 ? 1 : 0, quarter = warp & 3;
-    {
-      // Warps 2..5 stage Q, 6..9 dout: D/8 lanes to a row, chunk k of row r at k ^ (r & 7).
-      constexpr int LPR = D / 8, RPI = 32 / LPR;
-      uint8_t* dst = half ? sG : sQ;
-      const HeadStrides& ss = half ? a.os : a.qs;
-      const __nv_bfloat16* src = static_cast<const __nv_bfloat16*>(half ? p.g.dout : a.q) + b * ss.b;
-#pragma unroll 4
-      for (int i = 0; i < 32 / RPI; ++i) {
-        const int r = quarter * 32 + i * RPI + lane / LPR, c = lane % LPR;
-        const int g = (r0 + r) / a.q_len, t = (r0 + r) % a.q_len;
-        uint4 w = make_uint4(0, 0, 0, 0);
-        if (r0 + r < rows && t < q_end && c * 8 < a.d)
-          w = __ldg(reinterpret_cast<const uint4*>(src + (hk * group + g) * ss.h + t * ss.t + c * 8));
-        *reinterpret_cast<uint4*>(dst + (c >> 3) * CH + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = w;
-      }
-      fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&st->rows_full);
-    }
-    const int row = quarter * 32 + lane, rr = r0 + row;
-    const int g = rr / a.q_len, t = rr % a.q_len;
-    const bool store = rr < rows && t < q_end;
-    const long long term = (static_cast<long long>(b) * a.hq + hk * group + g) * p.q_pad + t;
-    const float nl = store ? p.neg_lse2[term] : -INFINITY, nd = store ? p.neg_d[term] : 0.0f;
-    const uint64_t sc2 = pk2(p.scale_log2, p.scale_log2), nl2 = pk2(nl, nl), nd2 = pk2(nd, nd);
-    const uint32_t lane_base = static_cast<uint32_t>(quarter * 32) << 16;
-    const uint32_t dp_tmem = tmem + lane_base + 256 + half * 64;
     bool ok = true;
-    unsigned char byte[4];
-    for (int j = 0; j < n; ++j) {
-      const int kv0 = j * TILE;
-      const bool partial = mask || kv0 + TILE > kv_end;
-      if (partial) load_mask_bytes(mask, kv0, kv_end, lane, byte);
-      if (!(ok = warp_wait_poll(&st->s_full[j & 1], (j >> 1) & 1, abort_flag, p.err, kErrCrossSoftmaxWait))) break;
-      tc_fence_after();
-      unsigned word[2] = {~0u, ~0u};
-      if (partial) {
-        const unsigned w0 = __ballot_sync(0xffffffffu, byte[0]), w1 = __ballot_sync(0xffffffffu, byte[1]);
-        const unsigned w2 = __ballot_sync(0xffffffffu, byte[2]), w3 = __ballot_sync(0xffffffffu, byte[3]);
-        word[0] = half ? w2 : w0;
-        word[1] = half ? w3 : w1;
-      }
-      uint64_t pr[32];
-#pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        uint32_t r[32];
-        tmem_ld32(tmem + lane_base + (j & 1) * 128 + half * 64 + c * 32, r);
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          float x0, x1;
-          unpk2(fma2(pk2(__uint_as_float(r[2 * e]), __uint_as_float(r[2 * e + 1])), sc2, nl2), x0, x1);
-          pr[c * 16 + e] = pk2(fast_exp2(x0), fast_exp2(x1));
+    int i = 0, x = 0;
+    for (int job = blockIdx.x; job < p.jobs && ok; job += grid) {
+      const Job<KV> j(p, job);
+      if (KV) {
+        if (j.count(a) == 0) {
+          // No query sees a key of this tile: zeros, a row's pieces to neighbouring lanes.
+          const int vecs = a.d / 8;
+          __nv_bfloat16* dk = static_cast<__nv_bfloat16*>(p.g.dk) + j.b * a.ks.b + j.hk * a.ks.h;
+          __nv_bfloat16* dv = static_cast<__nv_bfloat16*>(p.g.dv) + j.b * a.vs.b + j.hk * a.vs.h;
+          for (int k = lane; k < TILE * vecs; k += 32) {
+            const int key = j.r0 + k / vecs, c = k % vecs * 8;
+            if (key >= a.kv_len) break;
+            *reinterpret_cast<uint4*>(dk + key * a.ks.t + c) = make_uint4(0, 0, 0, 0);
+            *reinterpret_cast<uint4*>(dv + key * a.vs.t + c) = make_uint4(0, 0, 0, 0);
+          }
+          __syncwarp();
+          continue;
         }
-      }
-      if (!(ok = warp_wait_poll(&st->dp_full, j & 1, abort_flag, p.err, kErrCrossSoftmaxWait))) break;
-      tc_fence_after();
-#pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        uint32_t r[32], w[16];
-        tmem_ld32(dp_tmem + c * 32, r);
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          float x0, x1;
-          unpk2(mul2(pr[c * 16 + e], add2(pk2(__uint_as_float(r[2 * e]), __uint_as_float(r[2 * e + 1])), nd2)), x0, x1);
-          w[e] = pack_bf16x2(x0, x1);
-        }
-        if (partial) {  // a masked key's score or value may hold a NaN
-#pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            if (!((word[c] >> (2 * e)) & 1u)) w[e] &= 0xffff0000u;
-            if (!((word[c] >> (2 * e + 1)) & 1u)) w[e] &= 0x0000ffffu;
+        // The job's rows: into their boxes once the last ones have left them, or (X_SMEM) to where they stay once
+        // the last job is done.
+        uint64_t *const bar = L::X_SMEM ? &st->x_full[0] : &st->in_full, *const before = L::X_SMEM ? &st->done[0] : &st->in_free;
+        if (lane == 0) {
+          ok = x == 0 || mbar_wait_bounded_backoff(before, (x - 1) & 1, abort_flag, p.err, kErrCrossLoadWait, 32);
+          if (ok) {
+            uint8_t* box = smem + (L::X_SMEM ? L::X_OFF : L::IN_OFF);
+            mbar_arrive_expect_tx(bar, 2 * L::NCH * CH);
+            load_tile(box, &map_x1, L::NCH, j.r0, p.x1_head ? j.hk : 0, p.x1_batch ? j.b : 0, bar);
+            load_tile(box + L::NCH * CH, &map_x2, L::NCH, j.r0, p.x2_head ? j.hk : 0, p.x2_batch ? j.b : 0, bar);
           }
         }
-        tmem_st16(dp_tmem + c * 16, w);
+        ++x;
       }
-      tmem_wait_st();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&st->ds_full);
+      if (lane == 0)
+        for (int yb = j.b; yb < j.b_hi && ok; ++yb) {
+          const int y_end = j.span(a, yb);
+          for (int g = 0; g < j.heads && ok; ++g)
+            for (int t0 = 0; t0 < y_end; t0 += QT, ++i) {
+              const int s = i % NS;
+              if (i >= NS &&
+                  !mbar_wait_bounded_backoff(&st->free_[s], (i / NS - 1) & 1, abort_flag, p.err, kErrCrossLoadWait, 32)) {
+                ok = false;
+                break;
+              }
+              const int h = KV ? j.hk * j.group + g : j.hk;
+              mbar_arrive_expect_tx(&st->full[s], L::STAGE + (KV ? 512 : 0));
+              for (int c = 0; c < L::NCH; ++c)
+                tma_load_4d(sY1(s) + c * QCH, &map_y1, c * 64, t0, p.y1_head ? h : 0, p.y1_batch ? yb : 0, &st->full[s]);
+              for (int c = 0; c < L::NCH; ++c)
+                tma_load_4d(sY2(s) + c * QCH, &map_y2, c * 64, t0, p.y2_head ? h : 0, p.y2_batch ? yb : 0, &st->full[s]);
+              if (KV) {
+                const long long term = (static_cast<long long>(yb) * a.hq + h) * p.q_pad + t0;
+                bulk_load(terms(s), p.neg_lse2 + term, 256, &st->full[s]);
+                bulk_load(terms(s) + 64, p.neg_d + term, 256, &st->full[s]);
+              }
+            }
+        }
+      ok = __all_sync(0xffffffffu, ok);
     }
-    if (ok && n > 0) ok = warp_wait_poll(&st->done, 0, abort_flag, p.err, kErrCrossSoftmaxWait);
-    if (ok) {
+    if (!ok && lane == 0) {
+      for (int k = max(0, i - NS); k < i; ++k) drain_bar(&st->full[k % NS], (k / NS) & 1);
+      if (KV && x > 0) drain_bar(L::X_SMEM ? &st->x_full[0] : &st->in_full, (x - 1) & 1);
+    }
+  } else if (warp < 3) {
+    // ------------------------------------------------------------ S (warp 1) and dP (warp 2), whole warps
+    constexpr uint32_t IDESC = idesc_bf16_f32(TILE, QT, 0, 0);
+    const int which = warp - 1;
+    uint64_t *const read = which ? &st->dp_read : &st->s_read, *const ready = which ? st->dp_full : st->s_full;
+    const uint32_t col = tmem + (which ? L::DP : L::S);
+    bool ok = true;
+    const auto wait = [&](uint64_t* bar, uint32_t ph) {
+      return warp_wait_ready(bar, ph, abort_flag, p.err, kErrCrossMmaWait);
+    };
+    int i = 0, x = 0;
+    for (int job = blockIdx.x; job < p.jobs && ok; job += grid) {
+      const Job<KV> j(p, job);
+      const uint32_t rows = tmem + L::X + (x % NX) * L::XW + which * (D / 2);
+      bool first = true;
+      for (int yb = j.b; yb < j.b_hi && ok; ++yb) {
+        const int y_end = j.span(a, yb), y_len = KV ? a.q_len : a.kv_len;
+        const unsigned char* mask = !KV && a.key_mask ? a.key_mask + static_cast<long long>(yb) * a.kv_len : nullptr;
+        for (int g = 0; g < j.heads && ok; ++g)
+          for (int t0 = 0; t0 < y_end; t0 += QT, ++i) {
+            const int s = i % NS;
+            uint8_t* y = which ? sY2(s) : sY1(s);
+            if (first && !(ok = wait(&st->x_full[x % NX], (x / NX) & 1))) break;
+            first = false;
+            if (!(ok = wait(&st->full[s], (i / NS) & 1))) break;
+            // Rows that memory holds but that do not count are zeroed: their weights are 0, but a NaN
+            // would enter the sums all the same (Y2 of the dq walk, V, enters none).
+            if ((KV || !which) && (mask || (t0 + QT > y_end && y_end < y_len)))
+              scrub_rows<L::NCH, QT>(y, [&](int r) { return t0 + r < y_end && (!mask || mask[t0 + r]); });
+            if (i > 0 && !(ok = wait(read, (i - 1) & 1))) break;
+            tc_fence_after();
+            const uint64_t bd = smem_desc_sw128(smem_u32(y), 16, 1024);
+#pragma unroll
+            for (int c = 0; c < D / 64; ++c)
+              if constexpr (L::X_SMEM)
+                umma_f16_ss4_w(col, smem_desc_sw128(smem_u32(smem + L::X_OFF + (which * L::NCH + c) * CH), 16, 1024),
+                               bd + (c * QCH >> 4), IDESC, c > 0 ? 1u : 0u);
+              else
+                umma_f16_ts4k_w(col, rows + c * 32, bd + (c * QCH >> 4), IDESC, c > 0 ? 1u : 0u);
+            umma_commit_w(&ready[i & 1]);
+          }
+      }
+      if (!first) ++x;
+    }
+    if (!ok) {
+      umma_commit_w(&st->drain[which]);
+      drain_bar(&st->drain[which], 0);
+    }
+  } else if (warp == 3) {
+    // ------------------------------------------------------------ the sums (whole warp)
+    constexpr uint32_t IDESC = idesc_bf16_f32(TILE, D, 0, 1);  // Y MN-major
+    bool ok = true;
+    const auto wait = [&](uint64_t* bar, uint32_t ph) {
+      return warp_wait_ready(bar, ph, abort_flag, p.err, kErrCrossMmaWait);
+    };
+    int i = 0, x = 0;
+    for (int job = blockIdx.x; job < p.jobs && ok; job += grid) {
+      const int n = Job<KV>(p, job).count(a);
+      if (n == 0) continue;
+      const uint32_t sums = tmem + L::A + (x % NA) * L::AW;
+      if (x >= NA && !(ok = wait(&st->sums_free[x % NA], (x / NA - 1) & 1))) break;
+      for (int k = 0; k < n; ++k, ++i) {
+        const int s = i % NS, c = i & 1;
+        const uint32_t ph = (i >> 1) & 1, add = k > 0 ? 1u : 0u;
+        if (KV) {
+          if (!(ok = wait(&st->p_full[c], ph))) break;
+          tc_fence_after();
+          umma_f16_ts4_w(sums, tmem + L::P + c * 32, smem_desc_sw128(smem_u32(sY2(s)), QCH, 1024), IDESC, add);
+        }
+        if (!(ok = wait(&st->ds_full[c], ph))) break;
+        tc_fence_after();
+        umma_f16_ts4_w(sums + (KV ? D : 0), tmem + L::DS + c * 32, smem_desc_sw128(smem_u32(sY1(s)), QCH, 1024), IDESC, add);
+        umma_commit_w(&st->used[c]);
+        umma_commit_w(&st->free_[s]);
+      }
+      if (ok) umma_commit_w(&st->done[x % NA]);
+      ++x;
+    }
+    // No arrival may be in flight when the block ends: the last commits have landed when these have.
+    umma_commit_w(&st->drain[2]);
+    drain_bar(&st->drain[2], 0);
+  } else if (warp < 20) {
+    // ------------------------------------------------------------ P and dS
+    const int c = (warp - 4) >> 3, part = ((warp - 4) >> 2) & 1, quarter = warp & 3;
+    const int row = quarter * 32 + lane;
+    const uint32_t lanes = tmem + (static_cast<uint32_t>(quarter * 32) << 16);
+    const uint64_t sc2 = pk2(p.scale_log2, p.scale_log2);
+    bool ok = true;
+    int i0 = 0;  // items passed before this batch entry
+    for (int job = blockIdx.x; job < p.jobs && ok; job += grid) {
+      const Job<KV> j(p, job);
+      uint64_t nl2 = 0, nd2 = 0;
+      if (!KV) {
+        const int rr = j.r0 + row, t = rr % a.q_len;
+        const bool in = rr < j.group * a.q_len && t < cross_len(a.q_lens, j.b, a.q_len);
+        const long long term = (static_cast<long long>(j.b) * a.hq + j.hk * j.group + rr / a.q_len) * p.q_pad + t;
+        const float nl = in ? p.neg_lse2[term] : -INFINITY, nd = in ? p.neg_d[term] : 0.0f;
+        nl2 = pk2(nl, nl);
+        nd2 = pk2(nd, nd);
+      }
+      for (int yb = j.b; yb < j.b_hi && ok; ++yb) {
+        const int y_end = j.span(a, yb), n = j.heads * ((y_end + QT - 1) / QT);
+        const unsigned char* mask = a.key_mask ? a.key_mask + static_cast<long long>(yb) * a.kv_len : nullptr;
+        bool zero = false;  // KV: this row's key is masked
+        if (KV && n > 0) {
+          const int key = j.r0 + row;
+          zero = key >= cross_len(a.kv_lens, yb, a.kv_len) || (mask && !mask[key]);
+        }
+        for (int k = (i0 ^ c) & 1; k < n; k += 2) {
+          const int i = i0 + k, s = i % NS;
+          const uint32_t ph = (i >> 1) & 1;
+          const bool partial = !KV && (mask || k * QT + QT > y_end);
+          bool byte = true;  // of key k * 64 + part * 32 + lane
+          if (partial) {
+            const int key = k * QT + part * 32 + lane;
+            byte = key < y_end && (!mask || mask[key]);
+          }
+          if (KV && !(ok = warp_wait_ready(&st->full[s], (i / NS) & 1, abort_flag, p.err, kErrCrossSoftmaxWait))) break;
+          if (!(ok = warp_wait_ready(&st->s_full[c], ph, abort_flag, p.err, kErrCrossSoftmaxWait))) break;
+          tc_fence_after();
+          const float4* nl = reinterpret_cast<const float4*>(terms(s)) + part * 8;
+          uint32_t r[32], w[16];
+          uint64_t pr[16];  // this row's weights of 32 of the item's rows
+          tmem_ld32(lanes + L::S + part * 32, r);
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&st->s_read);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            uint64_t l0 = nl2, l1 = nl2;
+            if (KV) {
+              const float4 t = nl[e];
+              l0 = pk2(t.x, t.y);
+              l1 = pk2(t.z, t.w);
+            }
+            float x0, x1, x2, x3;
+            unpk2(fma2(pk2(__uint_as_float(r[4 * e]), __uint_as_float(r[4 * e + 1])), sc2, l0), x0, x1);
+            unpk2(fma2(pk2(__uint_as_float(r[4 * e + 2]), __uint_as_float(r[4 * e + 3])), sc2, l1), x2, x3);
+            x0 = fast_exp2(x0);
+            x1 = fast_exp2(x1);
+            x2 = fast_exp2(x2);
+            x3 = fast_exp2(x3);
+            pr[2 * e] = pk2(x0, x1);
+            pr[2 * e + 1] = pk2(x2, x3);
+            if (KV) {
+              w[2 * e] = zero ? 0u : pack_bf16x2(x0, x1);  // a masked key's scores may be anything
+              w[2 * e + 1] = zero ? 0u : pack_bf16x2(x2, x3);
+            }
+          }
+          // This group's P and dS of two items ago have been used.
+          if (i >= 2 && !(ok = warp_wait_ready(&st->used[c], ph ^ 1, abort_flag, p.err, kErrCrossSoftmaxWait))) break;
+          if (KV) {
+            tmem_st16(lanes + L::P + c * 32 + part * 16, w);
+            tmem_wait_st();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&st->p_full[c]);
+          }
+          if (!(ok = warp_wait_ready(&st->dp_full[c], ph, abort_flag, p.err, kErrCrossSoftmaxWait))) break;
+          tc_fence_after();
+          tmem_ld32(lanes + L::DP + part * 32, r);
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&st->dp_read);
+          const float4* nd = nl + 16;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            uint64_t d0 = nd2, d1 = nd2;
+            if (KV) {
+              const float4 t = nd[e];
+              d0 = pk2(t.x, t.y);
+              d1 = pk2(t.z, t.w);
+            }
+            float x0, x1, x2, x3;
+            unpk2(mul2(pr[2 * e], add2(pk2(__uint_as_float(r[4 * e]), __uint_as_float(r[4 * e + 1])), d0)), x0, x1);
+            unpk2(mul2(pr[2 * e + 1], add2(pk2(__uint_as_float(r[4 * e + 2]), __uint_as_float(r[4 * e + 3])), d1)), x2, x3);
+            w[2 * e] = zero ? 0u : pack_bf16x2(x0, x1);
+            w[2 * e + 1] = zero ? 0u : pack_bf16x2(x2, x3);
+          }
+          if (partial) {  // a masked key's score or value may hold a NaN
+            const unsigned word = __ballot_sync(0xffffffffu, byte);
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+              if (!((word >> (2 * e)) & 1u)) w[e] &= 0xffff0000u;
+              if (!((word >> (2 * e + 1)) & 1u)) w[e] &= 0x0000ffffu;
+            }
+          }
+          tmem_st16(lanes + L::DS + c * 32 + part * 16, w);
+          tmem_wait_st();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&st->ds_full[c]);
+        }
+        i0 += n;
+      }
+    }
+  } else {
+    // ------------------------------------------------------------ rows in, sums out
+    const int quarter = warp & 3, row = quarter * 32 + lane;
+    const uint32_t lanes = tmem + (static_cast<uint32_t>(quarter * 32) << 16);
+    bool ok = true;
+    // This thread's row of a job: offsets in X1 and X2, and in the gradients; false: there is no such row.
+    const auto row_at = [&](const Job<KV>& j, long long& o1, long long& o2) {
+      const int r = j.r0 + row;
+      if (KV) {
+        o1 = j.b * a.ks.b + j.hk * a.ks.h + r * a.ks.t;
+        o2 = j.b * a.vs.b + j.hk * a.vs.h + r * a.vs.t;
+        return r < a.kv_len;
+      }
+      const int h = j.hk * j.group + r / a.q_len, t = r % a.q_len;
+      o1 = j.b * a.qs.b + h * a.qs.h + t * a.qs.t;
+      o2 = j.b * a.os.b + h * a.os.h + t * a.os.t;
+      return r < j.group * a.q_len && t < cross_len(a.q_lens, j.b, a.q_len);
+    };
+    // Rows go through shared memory, so that eight lanes move 128 bytes of one: a lane to a row in global
+    // memory costs 32 transactions an access, and the warps that form P and dS wait behind them.
+    uint8_t *const in_box = smem + L::IN_OFF + quarter * 4096, *const out_box = smem + L::OUT_OFF + quarter * 4096;
+    const int sub = lane >> 3, piece = lane & 7;
+    const auto slot = [](uint8_t* box, int r, int k) {  // piece k of row r of a 128-byte-swizzled box
+      return reinterpret_cast<uint4*>(box + r * 128 + ((k ^ (r & 7)) << 4));
+    };
+    // Starts the copies of a job's rows into their boxes.  (Of keys' rows the TMA producer does.)
+    const auto fetch_rows = [&](const Job<KV>& j) {
+      if (KV) return;
+      long long o[2];
+      const bool in = row_at(j, o[0], o[1]);
+      const __nv_bfloat16* src[2] = {static_cast<const __nv_bfloat16*>(a.q), static_cast<const __nv_bfloat16*>(p.g.dout)};
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const long long at = __shfl_sync(0xffffffffu, in ? o[t] : -1, i * 4 + sub);
+#pragma unroll
+          for (int c = 0; c < D; c += 64) {
+            const int k = c + piece * 8;
+            const bool ok = at >= 0 && k < a.d;
+            cp_async16(slot(in_box + (t * L::NCH + c / 64) * CH, i * 4 + sub, piece), src[t] + (ok ? at + k : 0), ok);
+          }
+        }
+    };
+    // ... and puts them where the products read them: columns x % NX.
+    const auto place_rows = [&](int x) {
+      if constexpr (!L::X_SMEM) {
+        if (KV) {
+          if (!warp_wait_ready(&st->in_full, x & 1, abort_flag, p.err, kErrCrossLoadWait)) return;
+        } else {
+          cp_async_wait_all();
+          __syncwarp();
+        }
+#pragma unroll
+        for (int t = 0; t < 2 * L::NCH; ++t)
+#pragma unroll
+          for (int k = 0; k < 8; k += 4) {
+            uint32_t w[16];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const uint4 u = *slot(in_box + t * CH, lane, k + e);
+              w[4 * e] = u.x, w[4 * e + 1] = u.y, w[4 * e + 2] = u.z, w[4 * e + 3] = u.w;
+            }
+            tmem_st16(lanes + L::X + (x % NX) * L::XW + t * 32 + k * 4, w);
+          }
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(&st->x_full[x % NX]);
+          if (KV) mbar_arrive(&st->in_free);
+        }
+      }
+    };
+    // Zeros for rows whose sums are empty.  (Of keys' rows the TMA producer does.)
+    const auto store_zeros = [&](const Job<KV>& j) {
+      if (KV) return;
+      long long at, other;
+      const bool in = row_at(j, at, other);
+      for (int r = 0; r < 32; r += 4) {
+        const long long o = __shfl_sync(0xffffffffu, in ? at : -1, r + sub);
+        for (int c = piece * 8; o >= 0 && c < a.d; c += 64)
+          *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(p.g.dq) + o + c) = make_uint4(0, 0, 0, 0);
+        __syncwarp();
+      }
+    };
+    const auto next_job_quiet = [&](int job) {  // the next job with items, from `job` on
+      while (job < p.jobs && Job<KV>(p, job).count(a) == 0) job += grid;
+      return job;
+    };
+    const auto next_job = [&](int job) {  // the next one with items, from `job` on; zeros for those without
+      for (; job < p.jobs; job += grid) {
+        const Job<KV> j(p, job);
+        if (j.count(a) > 0) break;
+        store_zeros(j);
+      }
+      return job;
+    };
+    // The rows of the first NX jobs, then each time a job is done those of the one that takes its columns,
+    // fetched while it runs.
+    int x = 0, job = next_job(blockIdx.x);
+    int ahead = job;  // the next job to fetch
+    const auto advance = [&] { ahead = next_job(ahead + grid); };
+    for (int k = 0; k < NX && ahead < p.jobs; ++k) {
+      fetch_rows(Job<KV>(p, ahead));
+      place_rows(k);
+      advance();
+    }
+    while (job < p.jobs) {
+      if (!L::X_SMEM && ahead < p.jobs) fetch_rows(Job<KV>(p, ahead));
+      const Job<KV> j(p, job);
+      long long o[2];
+      const bool in = !KV && row_at(j, o[0], o[1]);
+      bool seen = true;
+      if (KV && (a.kv_lens || a.key_mask)) {  // a masked key's gradient is 0 whatever its row holds
+        seen = false;
+        for (int b = j.b; b < j.b_hi; ++b)
+          seen |= j.r0 + row < cross_len(a.kv_lens, b, a.kv_len) &&
+                  (!a.key_mask || a.key_mask[static_cast<long long>(b) * a.kv_len + min(j.r0 + row, a.kv_len - 1)]);
+      }
+      // (These warps wait long: they sleep between polls and leave the issue slots to the others.)
+      ok = mbar_wait_bounded_backoff(&st->done[x % NA], (x / NA) & 1, abort_flag, p.err, kErrCrossSoftmaxWait, 40);
+      if (!__all_sync(0xffffffffu, ok)) break;
       tc_fence_after();
-      __nv_bfloat16* out = static_cast<__nv_bfloat16*>(p.g.dq) + b * a.qs.b + (hk * group + g) * a.qs.h + t * a.qs.t;
+      if (NX == 1 && ahead < p.jobs) place_rows(x + 1);
+      // Sums: through the boxes, as many as there are at a time.
+      constexpr int SUMS = (KV ? 2 : 1) * L::NCH;  // chunks of 64 columns: dv, then dk; or dq
 #pragma unroll
-      for (int c0 = 0; c0 < D / 2; c0 += 32) {
-        const int c = half * (D / 2) + c0;  // each half stores half of the columns
-        uint32_t o[32];
-        tmem_ld32(tmem + lane_base + 384 + c, o);
-        if (store) {
+      for (int h0 = 0; h0 < SUMS; h0 += L::OUTS) {
+        if (KV && lane == 0) bulk_wait_group_read0();  // the boxes' last contents are on their way
+        __syncwarp();
 #pragma unroll
-          for (int e = 0; e < 32; e += 8)
-            if (c + e < a.d) {
+        for (int h = h0; h < h0 + L::OUTS; ++h) {
+          const float f = KV && h < L::NCH ? 1.0f : a.scale;  // dv has no scale
+#pragma unroll
+          for (int k = 0; k < 8; k += 4) {
+            uint32_t v[32];
+            __syncwarp();  // tcgen05.ld is warp-collective
+            tmem_ld32(lanes + L::A + (x % NA) * L::AW + h * 64 + k * 8, v);
+            if (h == SUMS - 1 && k == 4) {  // the last read: the columns take another job
+              tc_fence_before();
+              __syncwarp();
+              if (lane == 0) mbar_arrive(&st->sums_free[x % NA]);
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
               uint32_t w[4];
 #pragma unroll
               for (int q = 0; q < 4; ++q)
-                w[q] = n > 0 ? pack_bf16x2(__uint_as_float(o[e + 2 * q]) * a.scale,
-                                           __uint_as_float(o[e + 2 * q + 1]) * a.scale)
-                             : 0u;
-              *reinterpret_cast<uint4*>(out + c + e) = make_uint4(w[0], w[1], w[2], w[3]);
+                w[q] = seen ? pack_bf16x2(__uint_as_float(v[8 * e + 2 * q]) * f, __uint_as_float(v[8 * e + 2 * q + 1]) * f)
+                            : 0u;
+              *slot(out_box + (h - h0) * CH, lane, k + e) = make_uint4(w[0], w[1], w[2], w[3]);
             }
+          }
         }
-        __syncwarp();
+        if (KV) {
+          // 32 rows a box; the tensor maps end at kv_len and head_dim.
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0 && j.r0 + quarter * 32 < a.kv_len) {  // (no store starts past the tensor)
+            for (int h = h0; h < h0 + L::OUTS; ++h) {
+              const bool v = h < L::NCH;
+              tma_store_4d(v ? &map_dv : &map_dk, out_box + (h - h0) * CH, h % L::NCH * 64, j.r0 + quarter * 32,
+                           (v ? p.x2_head : p.x1_head) ? j.hk : 0, (v ? p.x2_batch : p.x1_batch) ? j.b : 0);
+            }
+            bulk_commit_group();
+          }
+        } else {
+          __syncwarp();
+#pragma unroll
+          for (int h = h0; h < h0 + L::OUTS; ++h) {
+            const int c = h * 64 + piece * 8;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              const long long at = __shfl_sync(0xffffffffu, in ? o[0] : -1, i * 4 + sub);
+              if (at >= 0 && c < a.d)
+                *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(p.g.dq) + at + c) =
+                    *slot(out_box + (h - h0) * CH, i * 4 + sub, piece);
+            }
+          }
+          __syncwarp();
+        }
       }
+      if (NX > 1 && ahead < p.jobs) place_rows(x + NX);
+      if (ahead < p.jobs) advance();
+      job = next_job_quiet(job + grid);
+      ++x;
     }
+    if (KV && lane == 0) bulk_wait_group0();  // shared memory outlives the stores' reads
   }
   tc_fence_before();
   __syncthreads();
@@ -1083,7 +1069,7 @@ using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t
                                    const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
                                    CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
 
-bool head_map(HeadMap* m, const void* base, const HeadStrides& s, int batch, int heads, int len, int d) {
+bool head_map(HeadMap* m, const void* base, const HeadStrides& s, int batch, int heads, int len, int d, int box_rows) {
   auto enc = reinterpret_cast<EncodeTiledFn>(tensor_map_encoder());
   if (!enc) return false;
   m->by_head = heads > 1 && s.h != 0;
@@ -1094,7 +1080,7 @@ bool head_map(HeadMap* m, const void* base, const HeadStrides& s, int batch, int
                               static_cast<cuuint64_t>(m->by_batch ? batch : 1)};
   const cuuint64_t strides[3] = {row, m->by_head ? static_cast<cuuint64_t>(s.h) * 2 : row,
                                  m->by_batch ? static_cast<cuuint64_t>(s.b) * 2 : row};
-  const cuuint32_t box[4] = {64, TILE, 1, 1}, estr[4] = {1, 1, 1, 1};
+  const cuuint32_t box[4] = {64, static_cast<cuuint32_t>(box_rows), 1, 1}, estr[4] = {1, 1, 1, 1};
   return enc(&m->map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(base), dims, strides, box, estr,
              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
@@ -1112,8 +1098,8 @@ cudaError_t fwd_tc(const CrossArgs& a, cudaStream_t s) {
   DeviceCtx* ctx = device_ctx();
   if (!ctx) return cudaErrorNoDevice;
   HeadMap mk, mv;
-  if (!head_map(&mk, a.k, a.ks, a.batch, a.hk, a.kv_len, a.d) ||
-      !head_map(&mv, a.v, a.vs, a.batch, a.hk, a.kv_len, a.d))
+  if (!head_map(&mk, a.k, a.ks, a.batch, a.hk, a.kv_len, a.d, TILE) ||
+      !head_map(&mv, a.v, a.vs, a.batch, a.hk, a.kv_len, a.d, TILE))
     return cudaErrorInvalidValue;
   static std::atomic<unsigned long long> attr{0};
   cudaError_t e = once_per_device(attr, [] {
@@ -1135,7 +1121,8 @@ cudaError_t fwd_tc(const CrossArgs& a, cudaStream_t s) {
 template <class Kernel>
 cudaError_t allow_smem(std::atomic<unsigned long long>& done, Kernel k, size_t bytes) {
   return once_per_device(done, [&] {
-    return cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes));
+    const cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes));
+    return e != cudaSuccess ? e : cudaFuncSetAttribute(k, cudaFuncAttributePreferredSharedMemoryCarveout, 100);
   });
 }
 
@@ -1144,33 +1131,42 @@ cudaError_t bwd_tc(const CrossGradArgs& g, const float* neg_lse2, const float* n
   const CrossArgs& a = g.f;
   DeviceCtx* ctx = device_ctx();
   if (!ctx) return cudaErrorNoDevice;
-  HeadMap mq, mg, mk, mv;
-  if (!head_map(&mq, a.q, a.qs, a.batch, a.hq, a.q_len, a.d) ||
-      !head_map(&mg, g.dout, a.os, a.batch, a.hq, a.q_len, a.d) ||
-      !head_map(&mk, a.k, a.ks, a.batch, a.hk, a.kv_len, a.d) ||
-      !head_map(&mv, a.v, a.vs, a.batch, a.hk, a.kv_len, a.d))
-    return cudaErrorInvalidValue;
-  const GradParams p{g,           neg_lse2,   neg_d,       q_pad,      mq.by_head,  mq.by_batch,         mg.by_head,
-                     mg.by_batch, mk.by_head, mk.by_batch, mv.by_head, mv.by_batch, a.scale * kLog2e, ctx->err_word};
-  if (g.dk) {
+  // One walk: resident blocks, one to an SM.
+  const auto walk = [&](auto kv, const HeadMap& y1, const HeadMap& y2, const HeadMap& x1, const HeadMap& x2,
+                        const HeadMap& dk, const HeadMap& dv, int tiles, int entries) -> cudaError_t {
+    constexpr bool KV = decltype(kv)::value;
+    using L = Grad<D, KV>;
     static std::atomic<unsigned long long> attr{0};
-    cudaError_t e = allow_smem(attr, cross_dkv_tc_kernel<D>, Dkv<D>::SMEM);
+    const cudaError_t e = allow_smem(attr, cross_grad_tc_kernel<D, KV>, L::SMEM);
     if (e != cudaSuccess) return e;
-    const long long blocks = static_cast<long long>((a.kv_len + TILE - 1) / TILE) * (g.kv_shared ? 1 : a.batch) * a.hk;
-    if (blocks > 0x7fffffffLL) return cudaErrorNotSupported;
-    cross_dkv_tc_kernel<D><<<static_cast<unsigned>(blocks), Dkv<D>::THREADS, Dkv<D>::SMEM, s>>>(mq.map, mg.map, mk.map,
-                                                                                              mv.map, p);
-    if ((e = cudaGetLastError()) != cudaSuccess) return e;
+    const long long jobs = static_cast<long long>(tiles) * entries * a.hk;
+    if (jobs > 0x7fffffffLL - ctx->sm_count) return cudaErrorNotSupported;
+    const GradParams p{g,           neg_lse2,   neg_d,       q_pad,      y1.by_head,  y1.by_batch,
+                       y2.by_head,  y2.by_batch, x1.by_head, x1.by_batch, x2.by_head, x2.by_batch,
+                       static_cast<int>(jobs), tiles, a.scale * kLog2e, ctx->err_word};
+    const unsigned blocks = static_cast<unsigned>(std::min<long long>(jobs, ctx->sm_count));
+    cross_grad_tc_kernel<D, KV><<<blocks, L::THREADS, L::SMEM, s>>>(y1.map, y2.map, x1.map, x2.map, dk.map, dv.map, p);
+    return cudaGetLastError();
+  };
+  HeadMap m1, m2, x1{}, x2{}, dk{}, dv{};
+  if (g.dk) {
+    const int entries = g.kv_shared ? 1 : a.batch;
+    if (!head_map(&m1, a.q, a.qs, a.batch, a.hq, a.q_len, a.d, QT) ||
+        !head_map(&m2, g.dout, a.os, a.batch, a.hq, a.q_len, a.d, QT) ||
+        !head_map(&x1, a.k, a.ks, entries, a.hk, a.kv_len, a.d, TILE) ||
+        !head_map(&x2, a.v, a.vs, entries, a.hk, a.kv_len, a.d, TILE) ||
+        !head_map(&dk, g.dk, a.ks, entries, a.hk, a.kv_len, a.d, 32) ||
+        !head_map(&dv, g.dv, a.vs, entries, a.hk, a.kv_len, a.d, 32))
+      return cudaErrorInvalidValue;
+    const cudaError_t e = walk(std::true_type{}, m1, m2, x1, x2, dk, dv, (a.kv_len + TILE - 1) / TILE, entries);
+    if (e != cudaSuccess) return e;
   }
   if (g.dq) {
-    static std::atomic<unsigned long long> attr{0};
-    cudaError_t e = allow_smem(attr, cross_dq_tc_kernel<D>, Dq<D>::SMEM);
+    if (!head_map(&m1, a.k, a.ks, a.batch, a.hk, a.kv_len, a.d, QT) ||
+        !head_map(&m2, a.v, a.vs, a.batch, a.hk, a.kv_len, a.d, QT))
+      return cudaErrorInvalidValue;
+    const cudaError_t e = walk(std::false_type{}, m1, m2, x1, x2, dk, dv, (a.hq / a.hk * a.q_len + TILE - 1) / TILE, a.batch);
     if (e != cudaSuccess) return e;
-    const long long rows = static_cast<long long>(a.hq / a.hk) * a.q_len;
-    const long long blocks = (rows + TILE - 1) / TILE * a.batch * a.hk;
-    if (blocks > 0x7fffffffLL) return cudaErrorNotSupported;
-    cross_dq_tc_kernel<D><<<static_cast<unsigned>(blocks), Dq<D>::THREADS, Dq<D>::SMEM, s>>>(mk.map, mv.map, p);
-    if ((e = cudaGetLastError()) != cudaSuccess) return e;
   }
   return cudaSuccess;
 }
