@@ -384,7 +384,34 @@ __device__ __forceinline__ bool warp_wait_poll(uint64_t* bar, uint32_t parity, v
 // the way.
 static __device__ __noinline__ bool warp_wait_slow(uint64_t* bar, uint32_t parity, volatile int* abort_flag,
                                                    unsigned* err_word, unsigned code) {
-  return warp_wait_poll(bar, parity, abort_flag, err_word, code);
+  // The hint lets the hardware hold the warp for up to 2 us a poll (it is woken when the phase completes), so
+  // a waiting warp takes no issue slots from the working ones.
+  const auto poll = [&] {
+    uint32_t ok;
+    asm volatile(
+        "{\n .reg .pred p;\n"
+        " mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n"
+        " selp.u32 %0, 1, 0, p;\n}\n"
+        : "=r"(ok)
+        : "r"(smem_u32(bar)), "r"(parity), "r"(2000u)
+        : "memory");
+    return ok != 0;
+  };
+  bool ok = true;
+  const uint64_t t0 = globaltimer_ns();
+  while (!poll()) {
+    if (*abort_flag) {
+      ok = false;
+      break;
+    }
+    if (globaltimer_ns() - t0 > LC_WAIT_TIMEOUT_NS) {
+      *abort_flag = 1;
+      if (err_word) atomicCAS(err_word, 0u, code);
+      ok = false;
+      break;
+    }
+  }
+  return __all_sync(0xffffffffu, ok);
 }
 __device__ __forceinline__ bool warp_wait_ready(uint64_t* bar, uint32_t parity, volatile int* abort_flag,
                                                 unsigned* err_word, unsigned code) {

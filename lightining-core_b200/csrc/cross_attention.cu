@@ -680,7 +680,13 @@ cudaError_t CrossSplitWork::begin(const CrossArgs& a, long long blocks, int tile
   DeviceCtx* ctx = device_ctx();
   if (!ctx) return cudaErrorNoDevice;
   const long long tiles = (a.kv_len + tile - 1) / tile, room = static_cast<long long>(per_sm) * ctx->sm_count;
-  const long long n = std::max(1LL, std::min<long long>({room / blocks, tiles, 64}));
+  return begin_parts(a, std::min<long long>({room / blocks, tiles, 64}), s);
+}
+
+cudaError_t CrossSplitWork::begin_parts(const CrossArgs& a, long long n, cudaStream_t s) {
+  DeviceCtx* ctx = device_ctx();
+  if (!ctx) return cudaErrorNoDevice;
+  n = std::max(1LL, n);
   sp.splits = static_cast<int>(n);
   sp.rows = static_cast<long long>(a.batch) * a.hq * a.q_len;
   sp.o = nullptr;
@@ -710,6 +716,7 @@ cudaError_t CrossSplitWork::end(const CrossArgs& a, cudaError_t e, cudaStream_t 
 }
 
 cudaError_t cross_attention_forward(const CrossArgs& a, cudaStream_t s) {
+  if (cross_few_supported(a)) return cross_forward_few(a, s);
   if (cross_tc_supported(a)) return cross_forward_tc(a, s);
   return a.bf16 ? fwd_simt_any<__nv_bfloat16>(a, s) : fwd_simt_any<float>(a, s);
 }

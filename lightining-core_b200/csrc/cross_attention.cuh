@@ -1,6 +1,8 @@
 // What the cross-attention kernels share.
 #pragma once
 
+#include <cuda.h>
+
 #include "lc_internal.hpp"
 
 namespace lcb {
@@ -24,6 +26,7 @@ struct CrossSplitWork {
   CrossSplit sp{};
   void* ws = nullptr;
   cudaError_t begin(const CrossArgs& a, long long blocks, int tile, int per_sm, cudaStream_t s);
+  cudaError_t begin_parts(const CrossArgs& a, long long n, cudaStream_t s);  // n parts (at most 1: none)
   cudaError_t end(const CrossArgs& a, cudaError_t launched, cudaStream_t s);
 };
 
@@ -31,6 +34,15 @@ struct CrossSplitWork {
 // alignment.
 bool cross_tc_supported(const CrossArgs& a);
 cudaError_t cross_forward_tc(const CrossArgs& a, cudaStream_t s);
+// Tensor maps of k and v in tiles of `rows` keys and 64 columns (128-byte swizzle), and which axes they have (an axis
+// that is not stepped over is one entry, its coordinate 0).
+struct KvAxes {
+  int k_head, k_batch, v_head, v_batch;
+};
+bool cross_kv_maps(const CrossArgs& a, int rows, CUtensorMap* k, CUtensorMap* v, KvAxes* ax);
+// At most 16 rows to a (batch, key head) pair (cross_attention_few.cu): head_dim 64 or 128.
+bool cross_few_supported(const CrossArgs& a);
+cudaError_t cross_forward_few(const CrossArgs& a, cudaStream_t s);
 // neg_lse2, neg_d: the row terms, [batch * q_heads][q_pad], q_pad whole tiles of 128 tokens.
 bool cross_grad_tc_supported(const CrossGradArgs& g);
 cudaError_t cross_backward_tc(const CrossGradArgs& g, const float* neg_lse2, const float* neg_d, int q_pad,

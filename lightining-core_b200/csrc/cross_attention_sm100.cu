@@ -1178,6 +1178,17 @@ bool cross_tc_supported(const CrossArgs& a) {
          rows16(a.v, a.vs, a.kv_len) && rows16(a.out, a.os, a.q_len) && tensor_map_encoder() != nullptr;
 }
 
+bool cross_kv_maps(const CrossArgs& a, int rows, CUtensorMap* k, CUtensorMap* v, KvAxes* ax) {
+  HeadMap mk, mv;
+  if (!head_map(&mk, a.k, a.ks, a.batch, a.hk, a.kv_len, a.d, rows) ||
+      !head_map(&mv, a.v, a.vs, a.batch, a.hk, a.kv_len, a.d, rows))
+    return false;
+  *k = mk.map;
+  *v = mv.map;
+  *ax = {mk.by_head, mk.by_batch, mv.by_head, mv.by_batch};
+  return true;
+}
+
 cudaError_t cross_forward_tc(const CrossArgs& a, cudaStream_t s) {
   return a.d <= 64 ? fwd_tc<64>(a, s) : fwd_tc<128>(a, s);
 }
