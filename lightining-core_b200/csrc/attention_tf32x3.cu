@@ -30,6 +30,7 @@
 #include <mutex>
 
 #include "../../include/lc_b200.h"
+#include "attention_math.cuh"
 #include "common.cuh"
 #include "lc_internal.hpp"
 
@@ -87,19 +88,6 @@ struct Params {
   int cols;  // output columns: D, or proj_cols with a projection
   unsigned* err_word;
 };
-
-__device__ __forceinline__ float tf32_round(float x) {
-  uint32_t u = __float_as_uint(x);
-  if ((u & 0x7f800000u) != 0x7f800000u) u = (u + 0x1000u) & 0xffffe000u;
-  return __uint_as_float(u);
-}
-
-// 2^x, MUFU ex2 without flush-to-zero (relative error ~2^-22).
-__device__ __forceinline__ float exp2_acc(float x) {
-  float y;
-  asm("ex2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
 
 // ---- pre-pass -----------------------------------------------------------------------------------
 // Rows of 64 floats (unit u at src + u*unit_stride) -> contiguous hi/lo planes [units, S, 64],

@@ -718,6 +718,7 @@ cudaError_t CrossSplitWork::end(const CrossArgs& a, cudaError_t e, cudaStream_t 
 cudaError_t cross_attention_forward(const CrossArgs& a, cudaStream_t s) {
   if (cross_few_supported(a)) return cross_forward_few(a, s);
   if (cross_tc_supported(a)) return cross_forward_tc(a, s);
+  if (cross_f32_tc_supported(a)) return cross_forward_f32_tc(a, s);
   return a.bf16 ? fwd_simt_any<__nv_bfloat16>(a, s) : fwd_simt_any<float>(a, s);
 }
 

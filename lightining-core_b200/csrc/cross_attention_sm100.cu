@@ -366,7 +366,7 @@ __global__ void __launch_bounds__(Fwd<D>::THREADS, 1)
             float x0, x1, e0, e1;
             unpk2(fma2(pk2(__uint_as_float(r[g][2 * i]), __uint_as_float(r[g][2 * i + 1])), sc2, nm2), x0, x1);
             if ((i & 7) < 2) {
-              exp2_poly_pair(x0, x1, e0, e1);
+              exp2_poly_pair<4>(x0, x1, e0, e1);  // degree 3's 7.5e-5 would show in the lse of a row of few keys
             } else {
               e0 = fast_exp2(x0);
               e1 = fast_exp2(x1);

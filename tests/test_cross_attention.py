@@ -432,3 +432,27 @@ def test_host_arrays(gpu):
     b_out, _ = lc.cross_attention(lc.to_bf16(q), lc.to_bf16(k), lc.to_bf16(v), kv_lens=[50, 20], key_mask=mask,
                                   q_lens=[6, 2], dtype=lc.BF16)
     np.testing.assert_allclose(lc.from_bf16(b_out), want, atol=0.1)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,d,nq", [("bf16", 64, 70), ("bf16", 128, 70), ("bf16", 64, 1), ("f32", 64, 70), ("f32", 128, 3)])
+@pytest.mark.parametrize("nk", [1, 2, 5, 33])
+def test_log_sum_of_few_keys(gpu, dtype, d, nq, nk):
+    """lse with scores that are exact in any order (entries -1, 0, 1): what is left is the scale's and the
+    subtraction's rounding (|s| < 16 * log2 e: 2 * 2^-24 * 24), the exponential (2.7e-6), the sum (n u) and the
+    logarithm (2^-22 of a result below 8)."""
+    import torch
+    lc = gpu
+    g = torch.Generator(device="cuda").manual_seed(nk + nq)
+    t = torch.bfloat16 if dtype == "bf16" else torch.float32
+    pick = lambda *s: torch.randint(-1, 2, s, generator=g, device="cuda").to(t)
+    q, k, v = pick(2, 4, nq, d), pick(2, 2, nk, d), pick(2, 2, nk, d)
+    out, lse = torch.empty_like(q), torch.empty((2, 4, nq), device="cuda")
+    desc = lc.cross_attention_desc(2, 4, 2, nq, nk, d, lc.BF16 if dtype == "bf16" else lc.F32)
+    lc.check(lc.lib.lcCrossAttentionForward(desc, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(),
+                                            None, None))
+    s = torch.einsum("bhtd,bhnd->bhtn", q.double(), k.double().repeat_interleave(2, 1)) * d ** -0.5
+    assert s.abs().max() < 16
+    torch.cuda.synchronize()
+    off = (lse.double() - torch.logsumexp(s, -1)).abs().max().item()
+    assert off <= 48 * U + 2.7e-6 + nk * U + 8 * 4 * U
