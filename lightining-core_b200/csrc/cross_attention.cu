@@ -723,6 +723,7 @@ cudaError_t cross_attention_forward(const CrossArgs& a, cudaStream_t s) {
 }
 
 cudaError_t cross_attention_backward(const CrossGradArgs& g, cudaStream_t s) {
+  if (cross_grad_f32_tc_supported(g)) return cross_backward_f32_tc(g, s);
   return g.f.bf16 ? bwd_any<__nv_bfloat16>(g, s) : bwd_any<float>(g, s);
 }
 

@@ -34,9 +34,12 @@ struct CrossSplitWork {
 // alignment.
 bool cross_tc_supported(const CrossArgs& a);
 cudaError_t cross_forward_tc(const CrossArgs& a, cudaStream_t s);
-// fp32 on the tensor cores by the 3xTF32 split (cross_attention_tf32x3.cu): head_dim <= 64, 8 rows a pair or more.
+// fp32 on the tensor cores by the 3xTF32 split (cross_attention_tf32x3.cu): head_dim <= 128; forward from 8 rows a
+// pair on, backward where every batch entry has keys of its own.
 bool cross_f32_tc_supported(const CrossArgs& a);
 cudaError_t cross_forward_f32_tc(const CrossArgs& a, cudaStream_t s);
+bool cross_grad_f32_tc_supported(const CrossGradArgs& g);
+cudaError_t cross_backward_f32_tc(const CrossGradArgs& g, cudaStream_t s);
 // Tensor maps of k and v in tiles of `rows` keys and 64 columns (128-byte swizzle), and which axes they have (an axis
 // that is not stepped over is one entry, its coordinate 0).
 struct KvAxes {
