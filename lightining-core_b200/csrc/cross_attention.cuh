@@ -40,13 +40,15 @@ bool cross_f32_tc_supported(const CrossArgs& a);
 cudaError_t cross_forward_f32_tc(const CrossArgs& a, cudaStream_t s);
 bool cross_grad_f32_tc_supported(const CrossGradArgs& g);
 cudaError_t cross_backward_f32_tc(const CrossGradArgs& g, cudaStream_t s);
-// Tensor maps of k and v in tiles of `rows` keys and 64 columns (128-byte swizzle), and which axes they have (an axis
-// that is not stepped over is one entry, its coordinate 0).
+bool cross_rows16(const CrossArgs& a);
+// Tensor maps of k and v in tiles of `rows` keys and 128 bytes of columns (128-byte swizzle), and which axes they have
+// (an axis that is not stepped over is one entry, its coordinate 0).
 struct KvAxes {
   int k_head, k_batch, v_head, v_batch;
 };
 bool cross_kv_maps(const CrossArgs& a, int rows, CUtensorMap* k, CUtensorMap* v, KvAxes* ax);
-// At most 16 rows to a (batch, key head) pair (cross_attention_few.cu): head_dim 64 or 128.
+// Few rows to a (batch, key head) pair (cross_attention_few.cu): bf16 at most 16, head_dim 64 or 128; fp32 at most 8,
+// head_dim <= 128.
 bool cross_few_supported(const CrossArgs& a);
 cudaError_t cross_forward_few(const CrossArgs& a, cudaStream_t s);
 // neg_lse2, neg_d: the row terms, [batch * q_heads][q_pad], q_pad whole tiles of 128 tokens.

@@ -1069,27 +1069,23 @@ using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t
                                    const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
                                    CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
 
-bool head_map(HeadMap* m, const void* base, const HeadStrides& s, int batch, int heads, int len, int d, int box_rows) {
+// Boxes of 128 bytes (64 bf16 or, es = 4, 32 fp32 values) of box_rows tokens.
+bool head_map(HeadMap* m, const void* base, const HeadStrides& s, int batch, int heads, int len, int d, int box_rows,
+              int es = 2) {
   auto enc = reinterpret_cast<EncodeTiledFn>(tensor_map_encoder());
   if (!enc) return false;
   m->by_head = heads > 1 && s.h != 0;
   m->by_batch = batch > 1 && s.b != 0;
-  const cuuint64_t row = static_cast<cuuint64_t>(len > 1 ? s.t : d) * 2;
+  const cuuint64_t row = static_cast<cuuint64_t>(len > 1 ? s.t : d) * es;
   const cuuint64_t dims[4] = {static_cast<cuuint64_t>(d), static_cast<cuuint64_t>(len),
                               static_cast<cuuint64_t>(m->by_head ? heads : 1),
                               static_cast<cuuint64_t>(m->by_batch ? batch : 1)};
-  const cuuint64_t strides[3] = {row, m->by_head ? static_cast<cuuint64_t>(s.h) * 2 : row,
-                                 m->by_batch ? static_cast<cuuint64_t>(s.b) * 2 : row};
-  const cuuint32_t box[4] = {64, static_cast<cuuint32_t>(box_rows), 1, 1}, estr[4] = {1, 1, 1, 1};
-  return enc(&m->map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(base), dims, strides, box, estr,
+  const cuuint64_t strides[3] = {row, m->by_head ? static_cast<cuuint64_t>(s.h) * es : row,
+                                 m->by_batch ? static_cast<cuuint64_t>(s.b) * es : row};
+  const cuuint32_t box[4] = {static_cast<cuuint32_t>(128 / es), static_cast<cuuint32_t>(box_rows), 1, 1}, estr[4] = {1, 1, 1, 1};
+  return enc(&m->map, es == 2 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, const_cast<void*>(base), dims, strides, box, estr,
              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-}
-
-// 16-byte rows and strides that a tensor map can hold (below 2^40 bytes).
-bool rows16(const void* p, const HeadStrides& s, int len) {
-  const auto ok = [](long long x) { return x % 8 == 0 && x < (1LL << 38); };
-  return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ok(s.b) && ok(s.h) && ok(s.t) && (len == 1 || s.t != 0);
 }
 
 template <int D>
@@ -1173,15 +1169,24 @@ cudaError_t bwd_tc(const CrossGradArgs& g, const float* neg_lse2, const float* n
 
 }  // namespace
 
-bool cross_tc_supported(const CrossArgs& a) {
-  return a.bf16 && a.d <= 128 && a.d % 8 == 0 && rows16(a.q, a.qs, a.q_len) && rows16(a.k, a.ks, a.kv_len) &&
-         rows16(a.v, a.vs, a.kv_len) && rows16(a.out, a.os, a.q_len) && tensor_map_encoder() != nullptr;
+// 16-byte rows and strides that a tensor map can hold (below 2^40 bytes).
+bool cross_rows16(const CrossArgs& a) {
+  const int per = a.bf16 ? 8 : 4;  // values in 16 bytes
+  const auto ok = [&](const void* p, const HeadStrides& s, int len) {
+    const auto in = [&](long long x) { return x % per == 0 && x < (1LL << 37); };
+    return reinterpret_cast<uintptr_t>(p) % 16 == 0 && in(s.b) && in(s.h) && in(s.t) && (len == 1 || s.t != 0);
+  };
+  return a.d % per == 0 && ok(a.q, a.qs, a.q_len) && ok(a.k, a.ks, a.kv_len) && ok(a.v, a.vs, a.kv_len) &&
+         ok(a.out, a.os, a.q_len) && tensor_map_encoder() != nullptr;
 }
+
+bool cross_tc_supported(const CrossArgs& a) { return a.bf16 && a.d <= 128 && cross_rows16(a); }
 
 bool cross_kv_maps(const CrossArgs& a, int rows, CUtensorMap* k, CUtensorMap* v, KvAxes* ax) {
   HeadMap mk, mv;
-  if (!head_map(&mk, a.k, a.ks, a.batch, a.hk, a.kv_len, a.d, rows) ||
-      !head_map(&mv, a.v, a.vs, a.batch, a.hk, a.kv_len, a.d, rows))
+  const int es = a.bf16 ? 2 : 4;
+  if (!head_map(&mk, a.k, a.ks, a.batch, a.hk, a.kv_len, a.d, rows, es) ||
+      !head_map(&mv, a.v, a.vs, a.batch, a.hk, a.kv_len, a.d, rows, es))
     return false;
   *k = mk.map;
   *v = mv.map;

@@ -233,7 +233,7 @@ __device__ __forceinline__ void store_cols(float* out, const float* v, float f, 
 //               tagged shared-memory words and P_hi lies over S_j's columns; at D = 128 a tile has 32 keys, each
 //               warp reads them all and P_hi has columns of its own.
 // The tensor pipe bounds it: 1536 cycles a tile of 64 keys at D = 64.
-// B200, [4, 16, 333 x 1000, 64] with holes: 89 us, planes included (370 us on the CUDA cores).
+// B200, [4, 16, 333 x 1000, 64] with holes: 90 us, planes included (370 us on the CUDA cores); D = 128: 181 (698).
 template <int D>
 struct Fwd {
   static constexpr int T = 4096 / D, VS = D == 64 ? 2 : 1, OC = D / 2;
@@ -505,6 +505,8 @@ __global__ void __launch_bounds__(FWD_THREADS, 1)
 //           sums are folded
 //   warps 2..9  X into TMEM, then two warps to a row: P, dS, and a tile's sums folded into registers
 // The tensor pipe bounds it: 3072 cycles a tile of 64 rows for dk and dv at D = 64, 2304 for dq.
+// B200, [4, 16, 333 x 1000, 64]: 258 us, planes included (782 on the CUDA cores), D = 128: 608 (1852); one row a pair
+// 123 (226); [2, 8, 77 x 300, 64] 29 (84).
 enum GradPass { kGradDq, kGradDkv, kGradDk, kGradDv };
 
 template <int D>
@@ -944,9 +946,9 @@ cudaError_t bwd_f32(const CrossGradArgs& g, cudaStream_t s) {
 // (A grid's second axis ends at 65535.)
 bool cross_f32_tc_supported(const CrossArgs& a) {
   const long long rows = static_cast<long long>(a.hq / a.hk) * a.q_len, pairs = static_cast<long long>(a.batch) * a.hk;
-  // From 8 rows a pair on this beats the CUDA cores although most of the tile is padding: [4, 16, R x 1000, 64]
-  // takes 45 / 50 us for R = 8 / 128 here and 52 / 92 there; [16, 16, 512 x 16, 64] 77 and 94; one 64 x 64 tile 12.5
-  // both.
+  // From 8 rows a pair on (fewer go to the kernel of few rows, where their strides allow it) this beats the CUDA
+  // cores although most of the tile is padding: [4, 16, R x 1000, 64] takes 45 / 50 us for R = 8 / 128 here and
+  // 52 / 92 there, at 128 columns and R = 8 85 and 109; [16, 16, 512 x 16, 64] 77 and 94; one 64 x 64 tile 12.5 both.
   return !a.bf16 && a.d <= 128 && rows >= 8 && pairs <= 65535 && tensor_map_encoder() != nullptr;
 }
 
