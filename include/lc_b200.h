@@ -358,13 +358,15 @@ typedef struct lcCrossAttentionDesc {
  * queries and keys of different lengths, shared key heads, strides and masks.  A row without a visible
  * key is 0.  lse (fp32, dense [batch, q_heads, q_len], may be NULL) receives the log of each row's
  * sum of exp(scale * q k^T) (-infinity for a row without a visible key), which the backward pass needs.
- * f32: strict fp32 arithmetic; bf16: fp32 accumulation and softmax statistics; head_dim <= 256.
- * k and v may be broadcast over the batch (batch stride 0 with the other strides set: one source
+ * f32: fp32 arithmetic (on the tensor cores each product is the sum of three of its operands' high and low
+ * halves, off by 2^-22 of its magnitude at most; visible infinities come out as NaN there); bf16: fp32
+ * accumulation and softmax statistics, weights rounded to bf16; head_dim <= 256.  k and v may be broadcast over the batch (batch stride 0 with the other strides set: one source
  * for many targets).  `out` must not overlap itself or the inputs.
  * Policy as lcAttentionForward (NULL: device pointers, asynchronous; the output postprocess must be
  * neutral).  Host tensors are dense; q_lens follows upload_q, kv_lens and key_mask follow
- * upload_k, lse follows download_out.  Few queries over many keys are split along the keys, with a
- * stream-ordered workspace. */
+ * upload_k, lse follows download_out.  Stream-ordered workspaces: for few queries over many keys, which are
+ * split along the keys, and in f32 for the halves (twice the bytes of q, k and v at head_dim 64 or 128; where
+ * they do not fit, a slower path needs none). */
 lcError_t lcCrossAttentionForward(const lcCrossAttentionDesc* desc, const void* q, const void* k, const void* v,
                                   void* out, float* lse, const lcAttentionIoPolicy* policy, lcStream_t stream);
 
@@ -374,7 +376,9 @@ lcError_t lcCrossAttentionForward(const lcCrossAttentionDesc* desc, const void* 
  * heads of a key head and, when k and v are both broadcast over the batch, over the batch (one
  * [kv_heads, kv_len, head_dim] gradient); the other strides that would make two gradients share memory
  * are LC_INVALID_VALUE.  All sums are fp32 (or wider) in a fixed order: the same call gives the same
- * bits.  Device pointers, asynchronous on `stream`; allocates a stream-ordered workspace. */
+ * bits.  Device pointers, asynchronous on `stream`; allocates a stream-ordered workspace: 8 bytes a row and,
+ * in f32, the halves, of q, dout and k transposed too (8 times the bytes of q and 6 times those of k at
+ * head_dim 64 or 128). */
 lcError_t lcCrossAttentionBackward(const lcCrossAttentionDesc* desc, const void* dout, const void* q, const void* k,
                                    const void* v, const void* out, const float* lse, void* dq, void* dk, void* dv,
                                    lcStream_t stream);

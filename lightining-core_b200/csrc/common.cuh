@@ -477,22 +477,6 @@ __device__ __forceinline__ void umma_f16_ss4_w(uint32_t d_tmem, uint64_t a_desc,
       "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
       : "memory");
 }
-// The same with B MN-major (16 rows of 128 bytes = 128 descriptor units on).
-__device__ __forceinline__ void umma_f16_ss4n_w(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
-                                                uint32_t accumulate) {
-  asm volatile(
-      "{\n .reg .pred p, t, e;\n .reg .b64 a1, b1, a2, b2, a3, b3;\n"
-      " setp.ne.b32 p, %4, 0;\n setp.eq.b32 t, 0, 0;\n"
-      " add.s64 a1, %1, 2;\n add.s64 b1, %2, 128;\n add.s64 a2, %1, 4;\n add.s64 b2, %2, 256;\n"
-      " add.s64 a3, %1, 6;\n add.s64 b3, %2, 384;\n"
-      " elect.sync _|e, 0xffffffff;\n"
-      " @e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n"
-      " @e tcgen05.mma.cta_group::1.kind::f16 [%0], a1, b1, %3, t;\n"
-      " @e tcgen05.mma.cta_group::1.kind::f16 [%0], a2, b2, %3, t;\n"
-      " @e tcgen05.mma.cta_group::1.kind::f16 [%0], a3, b3, %3, t;\n}\n" ::"r"(d_tmem),
-      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
-      : "memory");
-}
 // The same with A in TMEM (16 bf16 values = 8 columns on per step) and B MN-major (16 rows of 128 bytes
 // = 128 descriptor units on).
 __device__ __forceinline__ void umma_f16_ts4_w(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc,

@@ -692,11 +692,12 @@ cudaError_t CrossSplitWork::begin_parts(const CrossArgs& a, long long n, cudaStr
   sp.o = nullptr;
   sp.ml = nullptr;
   if (n <= 1) return cudaSuccess;
-  const cudaError_t e =
-      workspace_alloc(ctx, &ws, static_cast<size_t>(n) * sp.rows * (a.d * sizeof(float) + sizeof(float2)), s);
+  const size_t stats = (static_cast<size_t>(n) * sp.rows + 1) / 2 * 2;  // the sums start on a 16-byte boundary
+  const cudaError_t e = workspace_alloc(
+      ctx, &ws, stats * sizeof(float2) + static_cast<size_t>(n) * sp.rows * a.d * sizeof(float), s);
   if (e != cudaSuccess) return e;
   sp.ml = static_cast<float2*>(ws);
-  sp.o = reinterpret_cast<float*>(sp.ml + n * sp.rows);
+  sp.o = reinterpret_cast<float*>(sp.ml + stats);
   return cudaSuccess;
 }
 
@@ -718,12 +719,20 @@ cudaError_t CrossSplitWork::end(const CrossArgs& a, cudaError_t e, cudaStream_t 
 cudaError_t cross_attention_forward(const CrossArgs& a, cudaStream_t s) {
   if (cross_few_supported(a)) return cross_forward_few(a, s);
   if (cross_tc_supported(a)) return cross_forward_tc(a, s);
-  if (cross_f32_tc_supported(a)) return cross_forward_f32_tc(a, s);
+  if (cross_f32_tc_supported(a)) {
+    const cudaError_t e = cross_forward_f32_tc(a, s);
+    if (e != cudaErrorMemoryAllocation) return e;
+    cudaGetLastError();  // no room for the split operands: the CUDA cores need none
+  }
   return a.bf16 ? fwd_simt_any<__nv_bfloat16>(a, s) : fwd_simt_any<float>(a, s);
 }
 
 cudaError_t cross_attention_backward(const CrossGradArgs& g, cudaStream_t s) {
-  if (cross_grad_f32_tc_supported(g)) return cross_backward_f32_tc(g, s);
+  if (cross_grad_f32_tc_supported(g)) {
+    const cudaError_t e = cross_backward_f32_tc(g, s);
+    if (e != cudaErrorMemoryAllocation) return e;
+    cudaGetLastError();
+  }
   return g.f.bf16 ? bwd_any<__nv_bfloat16>(g, s) : bwd_any<float>(g, s);
 }
 

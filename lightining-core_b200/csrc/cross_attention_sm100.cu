@@ -87,7 +87,12 @@ __device__ __forceinline__ void load_mask_bytes(const unsigned char* mask, int k
 //               thread owns a row (one TMEM lane) -- and the epilogue
 // TMEM: S_A 0, S_B 128, O_A 256, O_B 384; P_h is written as bf16 pairs over the first half of S_h
 // and read from there as the A operand.  O is rescaled only when a row's maximum grows by more than
-// 2^8 (the final division makes up for it).
+// 2^8 (the final division makes up for it).  P is rounded to bf16 for the second product, 2^-8 of a weight at most and
+// unbiased; the row's sum takes the unrounded weights.
+// Bound by the softmax warps: about 4500 cycles a pair of tiles at either head_dim, where the products take 1300 (64)
+// and 2200 (128).  A quarter of the exponentials on the FMA pipes keeps MUFU (16 a cycle) below that.  B200: [16,
+// 16, 512 x 2048 ragged, 64] 128 us, [8, 16/4, 2048 x 4096, 128] 530..600 us (1.04 to 0.92 PFLOP/s); the CUDA cores
+// took 1937 us and 22.6 ms.
 template <int D>
 struct Fwd {
   static constexpr int NCH = D / 64;
@@ -442,8 +447,9 @@ __global__ void __launch_bounds__(Fwd<D>::THREADS, 1)
 //   else  rows are queries as in the forward pass (X1 = Q, X2 = dout), items are keys (Y1 = K, Y2 = V):
 //         writes dq
 // With S = X1 Y1^T, P = exp(S - lse), dP = X2 Y2^T, dS = P (dP - D), the sums over the items are
-// A1 += P Y2 (dv) and A2 += dS Y1 (dk or dq), both kept in TMEM.  P and dS come out with a row per TMEM
-// lane and go to shared memory as the A operands; Y1 and Y2 are read as they lie, MN-major: nothing is
+// A1 += P Y2 (dv) and A2 += dS Y1 (dk or dq), both kept in TMEM.  P and dS are formed with a row per TMEM
+// lane, rounded to bf16 as the forward pass rounds its weights (the matrix unit's type; sums stay fp32), and go
+// back into TMEM columns of their own as the A operands; Y1 and Y2 are read as they lie, MN-major: nothing is
 // transposed.  Forming S and dP once for each side costs two products, 7 instead of 5; taking dq from the
 // walk that yields dk and dv would need atomics, whose order changes the result, or fp32 partial rows of
 // every key tile in memory.
@@ -452,14 +458,15 @@ __global__ void __launch_bounds__(Fwd<D>::THREADS, 1)
 // form P and dS; a wait and a commit cost the issuing warp some 100 cycles each.  Hence
 //   * X1 and X2 in TMEM as A operands: an N = 64 product then takes 36 cycles a step instead of 53 (its
 //     operands in shared memory are what binds it), and shared memory holds more items
-//   * P and dS in shared memory, so the score columns are free as soon as they have been read, and the next
-//     item's products run while this one's weights are formed
+//   * P and dS in columns of their own, so the score columns are free as soon as they have been read, and the
+//     next item's products run while this one's weights are formed (through shared memory instead, each warp's
+//     fence towards the matrix unit cost 600 cycles an item)
 //   * two groups of eight warps that take the items in turn
 //   * three issuing warps, for S, dP and the sums, which order each other by barriers only
 //   * resident blocks that go from job to job: four more warps load the next job's rows and store
 //     the last one's sums meanwhile (two sets of TMEM columns where they fit)
-// Before: blocks of one job each with one chain of products took 271 (head_dim 64) and 150 us (128) for dk and
-// dv at [16, 16, 512 x 2048 ragged, 64] and [4, 16/4, 1024 x 2048 ragged, 128], tensor pipe 27% and 52% active.
+// B200, row terms included: [16, 16, 512 x 2048 ragged, 64] 306 us (blocks of one job with one chain of products:
+// 471), [4, 16/4, 1024 x 2048 ragged, 128] 227 us (266).
 constexpr int QT = 64;         // rows of an item
 constexpr int QCH = QT * 128;  // one [64 rows x 64 bf16] box
 template <int D, bool KV>

@@ -960,7 +960,7 @@ bool cross_grad_f32_tc_supported(const CrossGradArgs& g) {
   const CrossArgs& a = g.f;
   const long long pairs = static_cast<long long>(a.batch) * a.hk;
   // (Keys that all batch entries share have one gradient: a sum over the batch, left to the CUDA cores.)
-  return !a.bf16 && a.d <= 128 && !g.kv_shared && pairs <= 65535 && tensor_map_encoder() != nullptr;
+  return !a.bf16 && a.d <= 128 && !(g.kv_shared && g.dk) && pairs <= 65535 && tensor_map_encoder() != nullptr;
 }
 
 cudaError_t cross_backward_f32_tc(const CrossGradArgs& g, cudaStream_t s) {

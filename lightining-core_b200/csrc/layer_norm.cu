@@ -7,9 +7,8 @@
 //   dgamma = sum over rows of dy * h,  dbeta = sum over rows of dy
 //
 // Both passes are bound by HBM: 8 and 14 operations for every value moved.  So a row is read once
-// and held in registers (as fp32 sums of its own type's values), by one warp while it has at most
-// 1024 columns and by up to eight warps (backward) or sixteen (forward) beyond that; every
-// statistic, sum and gradient accumulates in fp32 and is rounded once, on the way out.
+// and held in registers, by as many warps as it has 1024 columns (forward) or 512 (backward), up to 8192
+// columns; every statistic, sum and gradient accumulates in fp32 and is rounded once, on the way out.
 //
 // Weights' gradients: a thread owns the same columns in every row its block walks, so dgamma and
 // dbeta accumulate in its registers; a block adds its row groups in shared memory and writes one
@@ -115,20 +114,20 @@ __device__ __forceinline__ void group_sync(int id, int threads) {
   asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
 }
 
-// Both kernels give a row to W warps with kOwn columns a lane, several such groups to a block, one block
-// to an SM, and let a group walk rows.  What bounds them is bytes in flight: a group's rows arrive
+// The backward kernel gives a row to W warps with kBwdOwn columns a lane, several such groups to a block, one block
+// to an SM, and lets a group walk rows.  What bounds it is bytes in flight: a group's rows arrive
 // through a ring of its own in shared memory, filled by bulk copies several rows ahead, so ~150 KB
-// are under way to an SM whatever the registers hold, and the weights of a lane's columns (and, backward,
-// their gradients) stay in registers.  A row's stage is read into registers at once and handed to
-// the next copy at the row's first barrier.  Measured at [32768, 1024] bf16 backward (floor 31 us): 94 us
+// are under way to an SM whatever the registers hold, and the weights of a lane's columns and
+// their gradients stay in registers.  A row's stage is read into registers at once and handed to
+// the next copy at the row's first barrier.  Measured at [32768, 1024] bf16 (floor 31 us): 94 us
 // with a warp to a row, weights re-read and no ring; 54 us with a one-row register prefetch at 8
-// columns a lane, bound by issue slots; 16 columns a lane and packed fp32 pairs halve those.
+// columns a lane, bound by issue slots; 45 us so, with 16 columns a lane and packed fp32 pairs.
 // A copy starts on a 16-byte boundary: rows that do not are copied from the boundary before them to
-// the one after them (never into another page) and read from there with scalar accesses.
+// the one after them (never into another page) and read from there with scalar accesses: [5003, 1333]
+// fp32 27 us (floor 12).
 constexpr int kFwdOwn = 32, kBwdOwn = 16;     // columns a lane
 constexpr int kBwdWarps = 16;                 // of a block
-constexpr int kMaxWarps = 16;
-constexpr int kMaxCols = 8192;                // 16 warps to a row
+constexpr int kMaxCols = 8192;                // 16 warps to a row (backward)
 constexpr int kMaxStages = 8;
 constexpr size_t kRingBytes = 192 * 1024;
 
@@ -219,7 +218,7 @@ __device__ __forceinline__ float pair_sum(const uint64_t (&v)[4]) {
   return a + b;
 }
 
-// Adds a value (or a pair of them) over the W warps of a row; `buf` holds W of them and is not used
+// Adds a value over the W warps of a row; `buf` holds W of them and is not used
 // again before another barrier of the group.
 __device__ __forceinline__ float group_sum(float v, float* buf, int W, int wr, int lane, int bar) {
   v = warp_sum(v);
@@ -241,8 +240,8 @@ struct LnFwd {
 };
 
 struct NormTail {
-  uint64_t full[kMaxWarps * kMaxStages];
-  float2 sums[2][kMaxWarps];
+  uint64_t full[kBwdWarps * kMaxStages];
+  float2 sums[2][kBwdWarps];
   int abort_flag;
 };
 
@@ -346,21 +345,10 @@ __global__ void __launch_bounds__(512) ln_fwd_kernel(LnFwd a, int W) {
   }
 }
 
-// Sum over the W warps of a block; `buf` is W floats that nothing else uses.
-template <int W>
-__device__ __forceinline__ float row_sum(float v, float* buf, int warp_in_row, int lane, int bar_id) {
-  v = warp_sum(v);
-  if (lane == 0) buf[warp_in_row] = v;
-  group_sync(bar_id, W * 32);
-  float t = 0.0f;
-#pragma unroll
-  for (int i = 0; i < W; ++i) t += buf[i];
-  return t;
-}
-
+// Sum over a block's warps; `buf` is a float for each that nothing else uses.
 template <int THREADS>
 __device__ __forceinline__ float block_sum(float v, float* buf) {
-  return row_sum<THREADS / 32>(v, buf, threadIdx.x >> 5, threadIdx.x & 31, 1);
+  return group_sum(v, buf, THREADS / 32, threadIdx.x >> 5, threadIdx.x & 31, 1);
 }
 
 // Rows too long for registers: one block streams the row three times (L2 serves the re-reads).
@@ -434,7 +422,7 @@ __global__ void __launch_bounds__(kBwdWarps * 32, 1) ln_bwd_kernel(LnBwd a, Rows
   bool ok = true;
   T* dx = static_cast<T*>(a.dx) + row * a.dx_stride;
   float2* sums = tail.sums[0] + group * W;  // alternates between the two sets
-  int other = kMaxWarps;
+  int other = kBwdWarps;
   for (; row < a.rows; row += hop, dx += hop * a.dx_stride, sums += other, other = -other, ring.step()) {
     const float r = rstd;
     const uint64_t r2 = pk2(r, r), nm = pk2(-mean, -mean);
@@ -588,14 +576,14 @@ __global__ void __launch_bounds__(32 * kRedSlices) ln_reduce_kernel(const float*
 
 bool aligned(const void* p, size_t bytes) { return (reinterpret_cast<uintptr_t>(p) % bytes) == 0; }
 
-// The split of `tensors` staged tensors of rows over a block: as many rows to a block as 16 warps hold,
-// but no more than spread the rows over all SMs; rings of up to 8 rows.
-Rows rows_of(size_t rows, size_t cols, int es, int tensors, int own, int warps, int sms) {
+// The split of the backward pass over a block: as many rows to a block as 16 warps hold, but no more than spread
+// the rows over all SMs; rings of up to 8 rows of x and dout.
+Rows rows_of(size_t rows, size_t cols, int es, int sms) {
   Rows r;
-  r.warps = static_cast<int>((cols + 32 * own - 1) / (32 * own));
-  r.groups = static_cast<int>(std::min<size_t>(warps / r.warps, (rows + sms - 1) / sms));
+  r.warps = static_cast<int>((cols + 32 * kBwdOwn - 1) / (32 * kBwdOwn));
+  r.groups = static_cast<int>(std::min<size_t>(kBwdWarps / r.warps, (rows + sms - 1) / sms));
   r.pitch = static_cast<int>((cols * es + 30 + 15) / 16 * 16);
-  const size_t row_bytes = static_cast<size_t>(r.pitch) * tensors * r.groups;
+  const size_t row_bytes = static_cast<size_t>(r.pitch) * 2 * r.groups;
   r.stages = static_cast<int>(std::min<size_t>(kMaxStages, kRingBytes / row_bytes));
   return r;
 }
@@ -647,7 +635,7 @@ cudaError_t ln_bwd(LnBwd a, void* dgamma, void* dbeta, int param_bf16, cudaStrea
   a.err = ctx->err_word;
   const bool in_regs = a.cols <= static_cast<size_t>(kMaxCols);
   Rows rw{};
-  if (in_regs) rw = rows_of(a.rows, a.cols, sizeof(T), 2, kBwdOwn, kBwdWarps, ctx->sm_count);
+  if (in_regs) rw = rows_of(a.rows, a.cols, sizeof(T), ctx->sm_count);
   // Blocks, each with a partial row of sums.
   const size_t per_block = in_regs ? rw.groups : 64;
   const int blocks = static_cast<int>(

@@ -456,3 +456,180 @@ def test_log_sum_of_few_keys(gpu, dtype, d, nq, nk):
     torch.cuda.synchronize()
     off = (lse.double() - torch.logsumexp(s, -1)).abs().max().item()
     assert off <= 48 * U + 2.7e-6 + nk * U + 8 * 4 * U
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("size", [(1, 1, 1, 1, 13000, 64), (1, 1, 1, 1, 9000, 128), (1, 1, 1, 17, 3000, 64),
+                                  (1, 1, 1, 33, 1500, 128), (1, 3, 1, 1, 5000, 128), (1, 1, 1, 9, 2500, 200)])
+def test_odd_rows_split_over_the_keys(gpu, size, dtype):
+    """An odd number of rows in an odd number of parts: the parts' statistics and sums share a workspace."""
+    import torch
+    _both(torch, gpu, *size, dtype=dtype, keys="mask")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("d", [64, 128, 44])
+@pytest.mark.parametrize("hq,nq", [(2, 1), (4, 1), (3, 1), (2, 4), (2, 5), (2, 8), (16, 1), (17, 1)])
+def test_row_counts_where_the_kernel_changes(gpu, dtype, d, hq, nq):
+    import torch
+    _both(torch, gpu, 3, hq, 1, nq, 190, d, dtype=dtype, keys="lens", queries="lens", layout="tokens")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,stride", [("bf16", 2 ** 32 + 64), ("f32", 2 ** 31 + 64)])
+@pytest.mark.parametrize("nq", [1, 40])
+@pytest.mark.parametrize("d", [64, 72])
+def test_offsets_past_32_bits(gpu, dtype, stride, nq, d):
+    """Batch entries of k, v and their gradients further apart than 32 bits reach, against the same values dense."""
+    import torch
+    lc, t = gpu, torch.bfloat16 if dtype == "bf16" else torch.float32
+    dt = lc.BF16 if dtype == "bf16" else lc.F32
+    b, h, nk = 2, 2, 150
+    g = torch.Generator(device="cuda").manual_seed(3)
+    near = [torch.randn((b, h, n, d), generator=g, device="cuda").to(t) for n in (nq, nq, nk, nk)]
+    q, do = near[:2]
+    far = []
+    for x in near[2:] + [near[2], near[3]]:
+        y = torch.as_strided(torch.empty(stride + h * nk * d, device="cuda", dtype=t), (b, h, nk, d), (stride, nk * d, d, 1))
+        y.copy_(x)
+        far.append(y)
+    got = []
+    for k, v, dk, dv, s in ((near[2], near[3], near[2].clone(), near[3].clone(), (h * nk * d, nk * d, d)),
+                            (*far, (stride, nk * d, d))):
+        o, dq, lse = torch.empty_like(q), torch.empty_like(q), torch.empty((b, h, nq), device="cuda")
+        desc = lc.cross_attention_desc(b, h, h, nq, nk, d, dt, k=s, v=s)
+        lc.check(lc.lib.lcCrossAttentionForward(desc, q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(),
+                                                lse.data_ptr(), None, None))
+        lc.check(lc.lib.lcCrossAttentionBackward(desc, do.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(),
+                                                 lse.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), None))
+        torch.cuda.synchronize()
+        got.append((o, lse, dq, dk, dv))
+    assert all(torch.equal(x, y) for x, y in zip(*got))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("nq,nk,d", [(1, 5000, 64), (2, 700, 128), (70, 2000, 64), (300, 300, 128)])
+def test_two_graphs_at_once(gpu, dtype, nq, nk, d):
+    """Two captured calls replayed on two streams at once do not share their workspaces."""
+    import torch
+    lc = gpu
+    cases, graphs, outs = [], [], []
+    for seed in (1, 2):
+        c, o, lse, grads = _both(torch, lc, 1, 2, 1, nq, nk, d, dtype=dtype, keys="mask", seed=seed)
+        gr = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(gr):
+            s = torch.cuda.current_stream().cuda_stream
+            o2, l2 = c.forward(s)
+            g2 = c.backward(o2, l2, stream=s)
+        cases.append((o, lse, *grads))
+        graphs.append(gr)
+        outs.append((o2, l2, *g2))
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    for _ in range(10):
+        for gr, st in zip(graphs, streams):
+            with torch.cuda.stream(st):
+                gr.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, y) for want, got in zip(cases, outs) for x, y in zip(want, got))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("d", [64, 128])
+def test_only_dq_with_a_shared_source(gpu, dtype, d):
+    import torch
+    c, o, lse, grads = _both(torch, gpu, 3, 4, 2, 30, 200, d, dtype=dtype, keys="lens", shared=True)
+    again = c.backward(o, lse, dkv=False)
+    torch.cuda.synchronize()
+    # Another kernel may serve this call: in fp32 each is off by at most (200 + 8) * 2^-22 of sums of magnitudes,
+    # which exceed the largest result by sqrt(200) or so.
+    off = float((again[0].double() - grads[0].double()).abs().max())
+    assert off <= (2 * 208 * 2.0 ** -22 * 15 * float(grads[0].double().abs().max()) if dtype == "f32" else 0.0)
+    assert bool((again[1].float() == HOLE).all()) and bool((again[2].float() == HOLE).all())
+
+
+def _block(torch, lc, x, mem, gamma, beta, w, dy, heads, lens, stream):
+    """Norm, projections and cross attention over `mem` as a decoder layer uses them, and the way back; every
+    tensor by token, [batch, tokens, columns].  Returns y and the gradients of x, gamma, beta, w and mem."""
+    b, n, c = x.shape
+    nk, d = mem.shape[1], c // heads
+    L, new = lc.lib, lambda *s: torch.empty(s, device="cuda")
+
+    def mm(a, bmat):
+        out = new(a.shape[0], bmat.shape[1])
+        lc.check(L.lcMatMul(a.data_ptr(), bmat.data_ptr(), out.data_ptr(), a.shape[0], a.shape[1], bmat.shape[1], lc.F32,
+                            None, stream))
+        return out
+
+    xf, mf, dyf = x.reshape(b * n, c), mem.reshape(b * nk, c), dy.reshape(b * n, c)
+    h, stats, lse = new(b * n, c), new(2, b * n), new(b, heads, n)
+    lc.check(L.lcLayerNormForward(xf.data_ptr(), gamma.data_ptr(), beta.data_ptr(), h.data_ptr(), stats[0].data_ptr(),
+                                  stats[1].data_ptr(), b * n, c, 0, 0, 1e-5, lc.F32, lc.F32, stream))
+    q, kv = mm(h, w["q"]), mm(mf, w["kv"])
+    k, v = kv, kv[:, c:]
+    by_q, by_k = (n * c, d, c), (nk * 2 * c, d, 2 * c)
+    desc = lc.cross_attention_desc(b, heads, heads, n, nk, d, lc.F32, by_q, by_k, by_k, by_q, kv_lens=lens.data_ptr())
+    o, dq, dkv, dx = new(b * n, c), new(b * n, c), new(b * nk, 2 * c), new(b * n, c)
+    lc.check(L.lcCrossAttentionForward(desc, q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), lse.data_ptr(), None,
+                                       stream))
+    y = mm(o, w["o"])
+    do = mm(dyf, w["o"].T.contiguous())
+    lc.check(L.lcCrossAttentionBackward(desc, do.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(),
+                                        lse.data_ptr(), dq.data_ptr(), dkv.data_ptr(), dkv[:, c:].data_ptr(), stream))
+    dh = mm(dq, w["q"].T.contiguous())
+    dgamma, dbeta = new(c), new(c)
+    lc.check(L.lcLayerNormBackward(dh.data_ptr(), xf.data_ptr(), gamma.data_ptr(), stats[0].data_ptr(), stats[1].data_ptr(),
+                                   dx.data_ptr(), dgamma.data_ptr(), dbeta.data_ptr(), b * n, c, 0, 0, 0, lc.F32, lc.F32,
+                                   stream))
+    return [y, dx, dgamma, dbeta, mm(h.T.contiguous(), dq), mm(mf.T.contiguous(), dkv), mm(o.T.contiguous(), dyf),
+            mm(dkv, w["kv"].T.contiguous())]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n,nk,heads,c", [(1, 33, 2, 64), (19, 70, 4, 256), (130, 200, 2, 256)])
+def test_a_decoder_layer(gpu, n, nk, heads, c):
+    """The operators together, eager and captured, on a stream of their own, against 64-bit autograd.  Tolerance:
+    seven stages one after the other, each off by at most (m + 8) * 2^-22 of its sums of magnitudes, m terms or fewer
+    (2^-22: the split of the fp32 products); sums of magnitudes exceed the results' largest by sqrt(m) or so."""
+    import torch
+    lc, b = gpu, 2
+    g = torch.Generator(device="cuda").manual_seed(n)
+    rnd = lambda *s: torch.randn(s, generator=g, device="cuda")
+    x, mem, dy = rnd(b, n, c), rnd(b, nk, c), rnd(b, n, c)
+    gamma, beta = 1 + 0.1 * rnd(c), 0.1 * rnd(c)
+    w = {"q": rnd(c, c) * c ** -0.5, "kv": rnd(c, 2 * c) * c ** -0.5, "o": rnd(c, c) * c ** -0.5}
+    lens = torch.tensor([nk, nk // 2 + 1], dtype=torch.int32, device="cuda")
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = _block(torch, lc, x, mem, gamma, beta, w, dy, heads, lens, side.cuda_stream)
+    torch.cuda.synchronize()
+    gr = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(gr):
+        again = _block(torch, lc, x, mem, gamma, beta, w, dy, heads, lens, torch.cuda.current_stream().cuda_stream)
+    for _ in range(2):
+        for t in again:
+            t.fill_(0)
+        gr.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(p, q) for p, q in zip(got, again))
+
+    leaves = [t.double().requires_grad_() for t in (x, gamma, beta, w["q"], w["kv"], w["o"], mem)]
+    x_, gm, bt, wq, wkv, wo, mem_ = leaves
+    h = torch.nn.functional.layer_norm(x_, (c,), gm, bt, 1e-5)
+    heads_of = lambda t: t.unflatten(-1, (heads, -1)).transpose(1, 2)
+    k, v = (mem_ @ wkv).chunk(2, -1)
+    s = heads_of(h @ wq) @ heads_of(k).transpose(-1, -2) * (c // heads) ** -0.5
+    hidden = torch.arange(nk, device="cuda")[None] >= lens[:, None]
+    p = torch.softmax(s.masked_fill(hidden[:, None, None, :], -float("inf")), -1)
+    y = (p @ heads_of(v)).transpose(1, 2).flatten(2) @ wo
+    gx, ggm, gbt, gq, gkv, go, gmem = torch.autograd.grad(y, leaves, dy.double())
+    want = [y, gx, ggm, gbt, gq, gkv, go, gmem]
+    m = max(c, b * n, b * nk)
+    for a, e in zip(got, want):
+        e = e.detach().reshape(a.shape)
+        assert float((a.double() - e).abs().max()) <= 7 * (m + 8) * 2.0 ** -22 * m ** 0.5 * float(e.abs().max())
