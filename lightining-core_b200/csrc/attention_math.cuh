@@ -42,27 +42,17 @@ __device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
 // and subtracting 1.5 * 2^23), f in [-0.5, 0.5]; 2^f by a degree-3 polynomial whose coefficients
 // are a weighted-least-squares minimax fit of 2^f on that interval (relative error 7.5e-5, far
 // below the bf16 rounding of P); 2^i is added into the exponent field.  x is clamped at -125 so
-// the result stays a normal number (a masked score gives 2^-125 instead of 0).  Degree 4 (error 2.7e-6,
-// Remez) serves where the row sum is an output of its own: a row of few keys shows one weight's error.
-template <int DEGREE = 3>
+// the result stays a normal number (a masked score gives 2^-125 instead of 0).
 __device__ __forceinline__ void exp2_poly_pair(float x0, float x1, float& y0, float& y1) {
-  static_assert(DEGREE == 3 || DEGREE == 4);
   constexpr float kRound = 12582912.0f;  // 1.5 * 2^23
   const uint64_t xx = pk2(fmaxf(x0, -125.0f), fmaxf(x1, -125.0f));
   const uint64_t t = add2(xx, pk2(kRound, kRound));
   const uint64_t r = add2(t, pk2(-kRound, -kRound));
   const uint64_t f = fma2(r, pk2(-1.0f, -1.0f), xx);
-  uint64_t q;
-  if constexpr (DEGREE == 3) {
-    q = fma2(pk2(0.05517132207751274f, 0.05517132207751274f), f, pk2(0.24261054396629333f, 0.24261054396629333f));
-    q = fma2(q, f, pk2(0.6932609677314758f, 0.6932609677314758f));
-    q = fma2(q, f, pk2(0.9999281167984009f, 0.9999281167984009f));
-  } else {
-    q = fma2(pk2(0.009570102207362652f, 0.009570102207362652f), f, pk2(0.05591785907745361f, 0.05591785907745361f));
-    q = fma2(q, f, pk2(0.240247443318367f, 0.240247443318367f));
-    q = fma2(q, f, pk2(0.6931217908859253f, 0.6931217908859253f));
-    q = fma2(q, f, pk2(0.9999992847442627f, 0.9999992847442627f));
-  }
+  uint64_t q = fma2(pk2(0.05517132207751274f, 0.05517132207751274f), f,
+                    pk2(0.24261054396629333f, 0.24261054396629333f));
+  q = fma2(q, f, pk2(0.6932609677314758f, 0.6932609677314758f));
+  q = fma2(q, f, pk2(0.9999281167984009f, 0.9999281167984009f));
   float q0, q1, t0, t1;
   unpk2(q, q0, q1);
   unpk2(t, t0, t1);

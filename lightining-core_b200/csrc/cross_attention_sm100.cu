@@ -78,21 +78,23 @@ __device__ __forceinline__ void load_mask_bytes(const unsigned char* mask, int k
 // ---- forward ----------------------------------------------------------------------------------
 // One block per SM owns two tiles of 128 rows (A and B) of a (batch, key head) pair, which share every
 // K and V tile of 128 keys.  A row is (head in the group, token), so short queries of a group fill a
-// tile together.  Roles (10 warps):
+// tile together.  Roles (18 warps):
 //   warp 0      TMA: K_j and V_j into rings of NS stages
 //   warp 1      MMA: S_h = Q_h K_j^T, O_h += P_h V_j for h = A, B, in the order PV_A(j), S_A(j+1),
 //               PV_B(j), S_B(j+1), so that one tile's softmax runs beside the other's products;
 //               it also zeroes the masked rows of V_j
-//   warps 2..5  rows of A (warps 6..9: of B): the Q rows into shared memory, then softmax -- a
-//               thread owns a row (one TMEM lane) -- and the epilogue
-// TMEM: S_A 0, S_B 128, O_A 256, O_B 384; P_h is written as bf16 pairs over the first half of S_h
-// and read from there as the A operand.  O is rescaled only when a row's maximum grows by more than
+//   warps 2..9  rows of A (warps 10..17: of B): the Q rows into shared memory, then softmax -- two threads
+//               to a row (one TMEM lane), 64 keys of a tile and half of the output columns each, which
+//               swap the row's maximum through tagged words in shared memory -- and the epilogue
+// TMEM: S_A 0, S_B 128.  At head_dim 64 P_A 256, P_B 320, O_A 384, O_B 448, and S_h(j+1) is issued when S_h(j) is in
+// the softmax warps' registers; at 128 O_A 256, O_B 384 leave P_h (bf16 pairs) to lie over the first half of S_h.  O is rescaled only when a row's maximum grows by more than
 // 2^8 (the final division makes up for it).  P is rounded to bf16 for the second product, 2^-8 of a weight at most and
 // unbiased; the row's sum takes the unrounded weights.
-// Bound by the softmax warps: about 4500 cycles a pair of tiles at either head_dim, where the products take 1300 (64)
-// and 2200 (128).  A quarter of the exponentials on the FMA pipes keeps MUFU (16 a cycle) below that.  B200: [16,
-// 16, 512 x 2048 ragged, 64] 128 us, [8, 16/4, 2048 x 4096, 128] 530..600 us (1.04 to 0.92 PFLOP/s); the CUDA cores
-// took 1937 us and 22.6 ms.
+// Bound by the issue slots and dependent steps of the softmax warps: about 3500 cycles a pair of tiles at head_dim 64
+// (MUFU 2048 of them, the products 1130) and 4500 at 128, where S, P and the sums of a tile follow one another (2200).
+// B200: [16, 16, 512 x 2048 ragged, 64] 111 us, [8, 16/4, 2048 x 4096, 128] 528 us (1.04 PFLOP/s); the CUDA cores
+// took 1937 us and 22.6 ms.  At 64, one issuing warp and P over S took 127; one thread to a row (8 warps fewer) 116;
+// a fourth of the exponentials by a polynomial on the FMA pipes, which pays in the self attention kernel, 113.
 template <int D>
 struct Fwd {
   static constexpr int NCH = D / 64;
@@ -101,17 +103,20 @@ struct Fwd {
   static constexpr int K_OFF = 2 * BYTES;
   static constexpr int V_OFF = K_OFF + NS * BYTES;
   static constexpr int TAIL_OFF = V_OFF + NS * BYTES;
-  static constexpr int THREADS = 320;
+  static constexpr int THREADS = 608;
   struct Tail {
-    uint64_t q_full[2];             // 4 warp arrivals
+    unsigned long long swap[2][2][2][TILE];  // [tile][step & 1][half][row], tagged with the step
+    uint64_t q_full[2];             // 8 warp arrivals
     uint64_t k_full[NS], v_full[NS];
     uint64_t k_free[NS], v_free[NS];
-    uint64_t s_full[2], p_full[2], o_done[2];
-    uint64_t drain;
+    uint64_t s_full[2], s_read[2], p_full[2], o_done[2];
+    uint64_t stagger, drain[2];  // stagger: A is half way through its first step (8 warp arrivals)
     uint32_t tmem_base;
     int abort_flag;
   };
   static constexpr size_t SMEM = 1024 + TAIL_OFF + sizeof(Tail);
+  static constexpr bool OWN_P = D == 64;  // P has columns of its own
+  static constexpr uint32_t P_COL = OWN_P ? 256 : 0, P_STEP = OWN_P ? 64 : 128, O_COL = OWN_P ? 384 : 256, O_STEP = D;
 };
 constexpr float kRescale = 8.0f;
 
@@ -166,17 +171,20 @@ __global__ void __launch_bounds__(Fwd<D>::THREADS, 1)
       mbar_init(&st->v_free[s], 1);
     }
     for (int h = 0; h < 2; ++h) {
-      mbar_init(&st->q_full[h], 4);
+      mbar_init(&st->q_full[h], 8);
       mbar_init(&st->s_full[h], 1);
-      mbar_init(&st->p_full[h], 4);
+      mbar_init(&st->s_read[h], 8);
+      mbar_init(&st->p_full[h], 8);
       mbar_init(&st->o_done[h], 1);
     }
-    mbar_init(&st->drain, 1);
+    mbar_init(&st->stagger, 8);
+    for (int i = 0; i < 2; ++i) mbar_init(&st->drain[i], 1);
     st->abort_flag = 0;
     fence_barrier_init();
     tma_prefetch_desc(&map_k);
     tma_prefetch_desc(&map_v);
   }
+  for (int i = threadIdx.x; i < 8 * TILE; i += F::THREADS) (&st->swap[0][0][0][0])[i] = ~0ull;
   if (warp == 0) {
     tmem_alloc(&st->tmem_base, 512);
     tmem_relinquish();
@@ -216,13 +224,13 @@ __global__ void __launch_bounds__(Fwd<D>::THREADS, 1)
         for (int j = max(0, v_issued - NS); j < v_issued; ++j) drain_bar(&st->v_full[j % NS], (j / NS) & 1);
       }
     }
-  } else if (warp == 1) {
-    // ------------------------------------------------------------ MMA issuer (whole warp)
+  } else if (warp == 1 || warp == 18) {
+    // ------------------------------------------------------------ MMA issuers (whole warps)
     constexpr uint32_t IDESC_S = idesc_bf16_f32(TILE, TILE, 0, 0);  // Q and K K-major
     constexpr uint32_t IDESC_O = idesc_bf16_f32(TILE, D, 0, 1);     // P in TMEM, V MN-major
     bool ok = true, issued = false;
     const auto wait = [&](uint64_t* bar, uint32_t ph) {
-      return warp_wait_poll(bar, ph, abort_flag, p.err, kErrCrossMmaWait);
+      return warp_wait_ready(bar, ph, abort_flag, p.err, kErrCrossMmaWait);
     };
     const auto issue_s = [&](int h, int j) {
       const uint64_t qd = smem_desc_sw128(smem_u32(sQ(h)), 16, 1024);
@@ -235,52 +243,80 @@ __global__ void __launch_bounds__(Fwd<D>::THREADS, 1)
     };
     const auto issue_pv = [&](int h, int j) {
       const uint64_t vd = smem_desc_sw128(smem_u32(sV(j % NS)), CH, 1024);
-      umma_f16_ts4_w(tmem + 256 + h * 128, tmem + h * 128, vd, IDESC_O, j > 0 ? 1u : 0u);
-      umma_f16_ts4_w(tmem + 256 + h * 128, tmem + h * 128 + 32, vd + (4 * 2048 >> 4), IDESC_O, 1u);
+      const uint32_t o = tmem + F::O_COL + h * F::O_STEP, pr = tmem + F::P_COL + h * F::P_STEP;
+      umma_f16_ts4_w(o, pr, vd, IDESC_O, j > 0 ? 1u : 0u);
+      umma_f16_ts4_w(o, pr + 32, vd + (4 * 2048 >> 4), IDESC_O, 1u);
       umma_commit_w(&st->o_done[h]);
     };
-    if (n > 0) {
-      for (int h = 0; h < 2 && ok; ++h)
-        if (act[h]) {
-          ok = wait(&st->q_full[h], 0) && wait(&st->k_full[0], 0);
-          if (ok) {
-            tc_fence_after();
-            issue_s(h, 0);
-          }
-        }
-      if (ok && NS < n) umma_commit_w(&st->k_free[0]);
-    }
-    for (int j = 0; j < n && ok; ++j) {
+    // Scores of step j (their K tile has been waited for).
+    const auto scores = [&](int h, int j) {
+      tc_fence_after();
+      issue_s(h, j);
+    };
+    // Weights of step j times V; p_full[h] next completes for P_h(j+1), which needs what is issued after this wait.
+    const auto sums = [&](int h, int j) {
+      if (!wait(&st->p_full[h], j & 1)) return false;
+      tc_fence_after();
+      issue_pv(h, j);
+      issued = true;
+      return true;
+    };
+    // V of step j, its masked rows zeroed: keys past kv_end that memory holds (TMA zero-fills past kv_len), and holes.
+    const auto values = [&](int j) {
       const int s = j % NS, kv0 = (t_lo + j) * TILE;
-      if (!(ok = wait(&st->v_full[s], (j / NS) & 1))) break;
-      // Masked rows of V: keys past kv_end that memory holds (TMA zero-fills past kv_len), and holes.
+      if (!wait(&st->v_full[s], (j / NS) & 1)) return false;
       if (mask || (kv0 + TILE > kv_end && kv_end < a.kv_len))
         scrub_rows<F::NCH, TILE>(sV(s), [&](int r) { return kv0 + r < kv_end && (!mask || mask[kv0 + r]); });
+      return true;
+    };
+    if (n > 0 && warp == 1) {
       for (int h = 0; h < 2 && ok; ++h) {
         if (!act[h]) continue;
-        // p_full[h] next completes for P_h(j+1), which needs S_h(j+1), issued after this wait.
-        if (!(ok = wait(&st->p_full[h], j & 1))) break;
-        tc_fence_after();
-        issue_pv(h, j);
-        if (j + 1 < n) {
-          if (!(ok = wait(&st->k_full[(j + 1) % NS], ((j + 1) / NS) & 1))) break;
-          tc_fence_after();
-          issue_s(h, j + 1);
-        }
+        if (F::OWN_P && h == 1 && act[0]) ok = wait(&st->stagger, 0);
+        if (ok && (ok = wait(&st->q_full[h], 0) && wait(&st->k_full[0], 0))) scores(h, 0);
       }
-      if (!ok) break;
-      // Both commits cover everything issued so far: the last readers of V_j and of K_{j+1}.  Only
-      // stages that are loaded again are handed back, so no arrival is left in flight at the end.
-      if (j + NS < n) umma_commit_w(&st->v_free[s]);
-      if (j + 1 + NS < n) umma_commit_w(&st->k_free[(j + 1) % NS]);
+      if (ok && NS < n) umma_commit_w(&st->k_free[0]);
+    }
+    // Commits cover everything issued so far, so one after both tiles' last product with a stage hands it back.
+    // Only stages that are loaded again are, so no arrival is left in flight at the end.
+    for (int j = 0; j < n && ok && (F::OWN_P || warp == 1); ++j) {
+      const auto k_used = [&] {
+        if (j + 1 + NS < n) umma_commit_w(&st->k_free[(j + 1) % NS]);
+      };
+      const auto next_keys = [&] { return j + 1 >= n || wait(&st->k_full[(j + 1) % NS], ((j + 1) / NS) & 1); };
+      if constexpr (F::OWN_P) {
+        // Tile B is half a step behind A (see stagger): one tile's exponentials run beside the rest of the
+        // other's softmax.
+        if (warp == 1) {
+          if (j + 1 == n || !(ok = next_keys())) break;
+          for (int h = 0; h < 2 && ok; ++h)  // s_read[h] next completes for S_h(j+1)
+            if (act[h] && (ok = wait(&st->s_read[h], j & 1))) scores(h, j + 1);
+          if (ok) k_used();
+        } else {
+          ok = values(j);
+          for (int h = 0; h < 2 && ok; ++h)
+            if (act[h]) ok = sums(h, j);
+          if (ok && j + NS < n) umma_commit_w(&st->v_free[j % NS]);
+        }
+      } else {
+        if (!(ok = values(j))) break;
+        for (int h = 0; h < 2 && ok; ++h) {
+          if (!act[h]) continue;
+          if (!(ok = sums(h, j) && next_keys())) break;
+          if (j + 1 < n) scores(h, j + 1);
+        }
+        if (!ok) break;
+        if (j + NS < n) umma_commit_w(&st->v_free[j % NS]);
+        k_used();
+      }
     }
     if (!ok && issued) {
-      umma_commit_w(&st->drain);
-      drain_bar(&st->drain, 0);
+      umma_commit_w(&st->drain[warp & 1]);
+      drain_bar(&st->drain[warp & 1], 0);
     }
   } else {
     // ------------------------------------------------------------ rows of tile h
-    const int h = warp >= 6 ? 1 : 0;
+    const int h = warp >= 10 ? 1 : 0, half = ((warp - 2) >> 2) & 1;
     const int quarter = warp & 3;  // TMEM lanes a warp may read
     const int base = r0 + h * TILE;
     if (act[h]) {
@@ -289,8 +325,8 @@ __global__ void __launch_bounds__(Fwd<D>::THREADS, 1)
       uint8_t* q = sQ(h);
       const __nv_bfloat16* src = static_cast<const __nv_bfloat16*>(a.q) + b * a.qs.b;
 #pragma unroll 4
-      for (int i = 0; i < 32 / RPI; ++i) {
-        const int r = quarter * 32 + i * RPI + lane / LPR, c = lane % LPR;
+      for (int i = 0; i < 16 / RPI; ++i) {
+        const int r = quarter * 32 + half * 16 + i * RPI + lane / LPR, c = lane % LPR;
         const int g = (base + r) / a.q_len, t = (base + r) % a.q_len;
         uint4 w = make_uint4(0, 0, 0, 0);
         if (base + r < rows && t < q_end && c * 8 < a.d)
@@ -304,38 +340,68 @@ __global__ void __launch_bounds__(Fwd<D>::THREADS, 1)
       const int row = quarter * 32 + lane;  // = TMEM lane
       const uint32_t lane_base = static_cast<uint32_t>(quarter * 32) << 16;
       const uint32_t s_tmem = tmem + lane_base + static_cast<uint32_t>(h * 128);
-      const uint32_t o_tmem = s_tmem + 256;
+      const uint32_t p_tmem = tmem + lane_base + F::P_COL + h * F::P_STEP + half * 32;
+      const uint32_t o_tmem = tmem + lane_base + F::O_COL + h * F::O_STEP;
+      constexpr int OC = D / 2;
       float m = -INFINITY, l = 0.0f;
       bool ok = true;
-      unsigned char byte[4];
+      unsigned char byte[2];
+      // Publishes v under `tag` and fetches the other half's value of the same tag.  A slot is written again
+      // two steps later, when the partner, which has published the step between, has read it.  Both
+      // halves' scores are in registers by then: P may be written over them.
+      const auto swap = [&](uint32_t tag, float v, float* other) {
+        *reinterpret_cast<volatile unsigned long long*>(&st->swap[h][tag & 1][half][row]) =
+            (static_cast<unsigned long long>(tag) << 32) | __float_as_uint(v);
+        volatile unsigned long long* theirs = &st->swap[h][tag & 1][half ^ 1][row];
+        unsigned long long x = *theirs;
+        bool got = static_cast<uint32_t>(x >> 32) == tag;
+        if (!got) {
+          const uint64_t t0 = globaltimer_ns();
+          uint32_t spins = 0;
+          while (!(got = static_cast<uint32_t>((x = *theirs) >> 32) == tag)) {
+            if (*abort_flag) break;
+            if ((++spins & 63u) == 0 && globaltimer_ns() - t0 > LC_WAIT_TIMEOUT_NS) {
+              *abort_flag = 1;
+              atomicCAS(p.err, 0u, static_cast<unsigned>(kErrCrossSoftmaxWait));
+              break;
+            }
+          }
+        }
+        *other = __uint_as_float(static_cast<uint32_t>(x));
+        return __all_sync(0xffffffffu, got) != 0;
+      };
       for (int j = 0; j < n; ++j) {
-        const int kv0 = (t_lo + j) * TILE;
-        const bool partial = mask || kv0 + TILE > kv_end;
+        const int kv0 = (t_lo + j) * TILE + half * 64;
+        const bool partial = mask || kv0 + 64 > kv_end;
         if (partial) load_mask_bytes(mask, kv0, kv_end, lane, byte);
         // s_full[h] next completes for S_h(j+1), which needs P_h(j) from these warps first.
-        if (!(ok = warp_wait_poll(&st->s_full[h], j & 1, abort_flag, p.err, kErrCrossSoftmaxWait))) break;
+        if (!(ok = warp_wait_ready(&st->s_full[h], j & 1, abort_flag, p.err, kErrCrossSoftmaxWait))) break;
         tc_fence_after();
-        uint32_t r[4][32];
-#pragma unroll
-        for (int c = 0; c < 4; ++c) tmem_ld32(s_tmem + c * 32, r[c]);
+        uint32_t r[64];
+        tmem_ld64(s_tmem + half * 64, r);
+        if (F::OWN_P) {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&st->s_read[h]);
+        }
         if (partial) {
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {
+          for (int c = 0; c < 2; ++c) {
             const unsigned w = __ballot_sync(0xffffffffu, byte[c]);
 #pragma unroll
             for (int e = 0; e < 32; ++e)
-              if (!((w >> e) & 1u)) r[c][e] = __float_as_uint(-INFINITY);
+              if (!((w >> e) & 1u)) r[c * 32 + e] = __float_as_uint(-INFINITY);
           }
         }
         float pm[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) pm[i] = __uint_as_float(r[0][i]);
+        for (int i = 0; i < 8; ++i) pm[i] = __uint_as_float(r[i]);
 #pragma unroll
-        for (int e = 8; e < TILE; e += 2)
-          pm[(e >> 1) & 7] = max3(pm[(e >> 1) & 7], __uint_as_float(r[e >> 5][e & 31]),
-                                  __uint_as_float(r[(e + 1) >> 5][(e + 1) & 31]));
-        const float mx =
-            max3(max3(pm[0], pm[1], pm[2]), max3(pm[3], pm[4], pm[5]), fmaxf(pm[6], pm[7])) * p.scale_log2;
+        for (int e = 8; e < 64; e += 2)
+          pm[(e >> 1) & 7] = max3(pm[(e >> 1) & 7], __uint_as_float(r[e]), __uint_as_float(r[e + 1]));
+        float mx = max3(max3(pm[0], pm[1], pm[2]), max3(pm[3], pm[4], pm[5]), fmaxf(pm[6], pm[7])), mo;
+        if (!(ok = swap(static_cast<uint32_t>(j), mx, &mo))) break;
+        mx = fmaxf(mx, mo) * p.scale_log2;
         const bool need = mx > m + kRescale;
         float factor = 1.0f;
         if (need) {
@@ -343,13 +409,16 @@ __global__ void __launch_bounds__(Fwd<D>::THREADS, 1)
           l *= factor;
           m = mx;
         }
-        if (j > 0 && __any_sync(0xffffffffu, need)) {
-          // O_h is rescaled in place: PV_h(j-1) must have landed (o_done[h] next completes for
-          // PV_h(j), which needs this tile's P).
-          if (!(ok = warp_wait_poll(&st->o_done[h], (j - 1) & 1, abort_flag, p.err, kErrCrossSoftmaxWait))) break;
+        const bool rescale = __any_sync(0xffffffffu, need);
+        if (j > 0 && (rescale || F::OWN_P)) {
+          // O_h is rescaled in place, and columns of P's own are read by PV_h(j-1): it must have landed (o_done[h]
+          // next completes for PV_h(j), which needs this tile's P).
+          if (!(ok = warp_wait_ready(&st->o_done[h], (j - 1) & 1, abort_flag, p.err, kErrCrossSoftmaxWait))) break;
           tc_fence_after();
+        }
+        if (j > 0 && rescale) {
 #pragma unroll 1
-          for (int c = 0; c < D; c += 16) {
+          for (int c = half * OC; c < half * OC + OC; c += 16) {
             uint32_t o[16];
             tmem_ld16(o_tmem + c, o);
 #pragma unroll
@@ -358,28 +427,27 @@ __global__ void __launch_bounds__(Fwd<D>::THREADS, 1)
           }
           tmem_wait_st();
         }
-        // A row that has seen no key yet has m = -inf: every score is -inf too and its weights are 0
-        // (or 2^-125 where the polynomial serves, times rows of V that are zeros).
+        // A row that has seen no key yet has m = -inf: every score is -inf too and its weights are 0.
         const float mu = m == -INFINITY ? 0.0f : m;
         const uint64_t sc2 = pk2(p.scale_log2, p.scale_log2), nm2 = pk2(-mu, -mu);
         uint64_t ps2[4] = {0, 0, 0, 0};
 #pragma unroll
-        for (int g = 0; g < TILE / 32; ++g) {
+        for (int g = 0; g < 2; ++g) {
           uint32_t w[16];
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
             float x0, x1, e0, e1;
-            unpk2(fma2(pk2(__uint_as_float(r[g][2 * i]), __uint_as_float(r[g][2 * i + 1])), sc2, nm2), x0, x1);
-            if ((i & 7) < 2) {
-              exp2_poly_pair<4>(x0, x1, e0, e1);  // degree 3's 7.5e-5 would show in the lse of a row of few keys
-            } else {
-              e0 = fast_exp2(x0);
-              e1 = fast_exp2(x1);
-            }
+            unpk2(fma2(pk2(__uint_as_float(r[g * 32 + 2 * i]), __uint_as_float(r[g * 32 + 2 * i + 1])), sc2, nm2), x0, x1);
+            e0 = fast_exp2(x0);
+            e1 = fast_exp2(x1);
             ps2[i & 3] = add2(ps2[i & 3], pk2(e0, e1));
             w[i] = pack_bf16x2(e0, e1);
           }
-          tmem_st16(s_tmem + g * 16, w);
+          tmem_st16(p_tmem + g * 16, w);
+          if (F::OWN_P && g == 0 && j == 0 && h == 0) {
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&st->stagger);
+          }
         }
         float x, y;
         unpk2(add2(add2(ps2[0], ps2[1]), add2(ps2[2], ps2[3])), x, y);
@@ -390,8 +458,11 @@ __global__ void __launch_bounds__(Fwd<D>::THREADS, 1)
         if (lane == 0) mbar_arrive(&st->p_full[h]);
       }
       if (ok && n > 0)
-        ok = warp_wait_poll(&st->o_done[h], (n - 1) & 1, abort_flag, p.err, kErrCrossSoftmaxWait);
+        ok = warp_wait_ready(&st->o_done[h], (n - 1) & 1, abort_flag, p.err, kErrCrossSoftmaxWait);
+      float other = 0.0f;
+      if (ok && n > 0) ok = swap(static_cast<uint32_t>(n), l, &other);
       if (ok) {
+        l = half == 0 ? l + other : other + l;  // the same sum in both
         tc_fence_after();
         const int rr = base + row, g = rr / a.q_len, t = rr % a.q_len;
         const bool store = rr < rows && t < q_end;
@@ -399,14 +470,20 @@ __global__ void __launch_bounds__(Fwd<D>::THREADS, 1)
         const long long at = (static_cast<long long>(b) * a.hq + hk * group) * a.q_len + rr;  // dense row
         const bool split = p.sp.splits > 1;
         const float inv = split ? 1.0f : empty ? 0.0f : 1.0f / l;
-        if (store && split) p.sp.ml[static_cast<long long>(blockIdx.y) * p.sp.rows + at] = make_float2(m, empty ? 0.0f : l);
-        if (store && !split && a.lse) a.lse[at] = empty ? -INFINITY : (m + log2f(l)) * kLn2;
+        if (store && half == 0) {
+          if (split)
+            p.sp.ml[static_cast<long long>(blockIdx.y) * p.sp.rows + at] = make_float2(m, empty ? 0.0f : l);
+          else if (a.lse)
+            a.lse[at] = empty ? -INFINITY : (m + log2f(l)) * kLn2;
+        }
         float* part = p.sp.o + (static_cast<long long>(blockIdx.y) * p.sp.rows + at) * a.d;
         __nv_bfloat16* out = static_cast<__nv_bfloat16*>(a.out) + b * a.os.b + (hk * group + g) * a.os.h + t * a.os.t;
         // tcgen05.ld is warp-collective: every lane loads, only live rows store.
 #pragma unroll
-        for (int c = 0; c < D; c += 32) {
+        for (int cc = 0; cc < OC; cc += 32) {
+          const int c = half * OC + cc;
           uint32_t o[32];
+          __syncwarp();
           tmem_ld32(o_tmem + c, o);
 #pragma unroll
           for (int e = 0; e < 32; ++e)
@@ -426,7 +503,6 @@ __global__ void __launch_bounds__(Fwd<D>::THREADS, 1)
                 *reinterpret_cast<uint4*>(out + c + e) = make_uint4(w[0], w[1], w[2], w[3]);
               }
           }
-          __syncwarp();
         }
       }
     }
