@@ -63,14 +63,14 @@ __device__ __forceinline__ void scrub_rows(uint8_t* tile, Keep keep) {
   __syncwarp();
 }
 
-// Whether this lane's keys of the tile at kv0 (kv0 + 32 i + lane) are visible; a ballot of byte[i]
+// Whether this lane's keys of the tile at kv0 (kv0 + step i + lane) are visible; a ballot of byte[i]
 // gives every lane the word of those 32 keys.  Loaded ahead of the wait for the scores.
 template <int N>
 __device__ __forceinline__ void load_mask_bytes(const unsigned char* mask, int kv0, int kv_end, int lane,
-                                                unsigned char (&byte)[N]) {
+                                                unsigned char (&byte)[N], int step = 32) {
 #pragma unroll
   for (int i = 0; i < N; ++i) {
-    const int k = kv0 + i * 32 + lane;
+    const int k = kv0 + i * step + lane;
     byte[i] = k < kv_end && (!mask || mask[k]);
   }
 }
@@ -78,21 +78,24 @@ __device__ __forceinline__ void load_mask_bytes(const unsigned char* mask, int k
 // ---- forward ----------------------------------------------------------------------------------
 // One block per SM owns two tiles of 128 rows (A and B) of a (batch, key head) pair, which share every
 // K and V tile of 128 keys.  A row is (head in the group, token), so short queries of a group fill a
-// tile together.  Roles (18 warps):
+// tile together.  Roles (19 warps):
 //   warp 0      TMA: K_j and V_j into rings of NS stages
-//   warp 1      MMA: S_h = Q_h K_j^T, O_h += P_h V_j for h = A, B, in the order PV_A(j), S_A(j+1),
-//               PV_B(j), S_B(j+1), so that one tile's softmax runs beside the other's products;
-//               it also zeroes the masked rows of V_j
+//   warp 1      MMA: S_h = Q_h K_j^T, O_h += P_h V_j for h = A, B (at head_dim 128 in the order PV_A(j), S_A(j+1),
+//               PV_B(j), S_B(j+1)), so that one tile's softmax runs beside the other's products; the warp
+//               of the products with V also zeroes the masked rows of V_j
 //   warps 2..9  rows of A (warps 10..17: of B): the Q rows into shared memory, then softmax -- two threads
-//               to a row (one TMEM lane), 64 keys of a tile and half of the output columns each, which
-//               swap the row's maximum through tagged words in shared memory -- and the epilogue
-// TMEM: S_A 0, S_B 128.  At head_dim 64 P_A 256, P_B 320, O_A 384, O_B 448, and S_h(j+1) is issued when S_h(j) is in
-// the softmax warps' registers; at 128 O_A 256, O_B 384 leave P_h (bf16 pairs) to lie over the first half of S_h.  O is rescaled only when a row's maximum grows by more than
+//               to a row (one TMEM lane), 32 of every 64 keys of a tile and half of the output columns each,
+//               which swap the row's maximum through tagged words in shared memory -- and the epilogue
+//   warp 18     at head_dim 64: the products with V, while warp 1 issues the scores
+// TMEM: S_A 0, S_B 128.  At head_dim 64 P_A 256, P_B 320, O_A 384, O_B 448, and S_h(j+1) is issued when S_h(j)
+// is in the softmax warps' registers; at 128 O_A 256, O_B 384 leave P_h (bf16 pairs) to lie over the first half
+// of S_h.  The products with the first 64 weights of a step start while the other 64 are formed (at 128 509 us
+// instead of 527 below).  O is rescaled only when a row's maximum grows by more than
 // 2^8 (the final division makes up for it).  P is rounded to bf16 for the second product, 2^-8 of a weight at most and
 // unbiased; the row's sum takes the unrounded weights.
 // Bound by the issue slots and dependent steps of the softmax warps: about 3500 cycles a pair of tiles at head_dim 64
-// (MUFU 2048 of them, the products 1130) and 4500 at 128, where S, P and the sums of a tile follow one another (2200).
-// B200: [16, 16, 512 x 2048 ragged, 64] 111 us, [8, 16/4, 2048 x 4096, 128] 528 us (1.04 PFLOP/s); the CUDA cores
+// (MUFU 2048 of them, the products 1130) and 4300 at 128, where S, P and the sums of a tile follow one another (2200).
+// B200: [16, 16, 512 x 2048 ragged, 64] 111 us, [8, 16/4, 2048 x 4096, 128] 509 us (1.08 PFLOP/s); the CUDA cores
 // took 1937 us and 22.6 ms.  At 64, one issuing warp and P over S took 127; one thread to a row (8 warps fewer) 116;
 // a fourth of the exponentials by a polynomial on the FMA pipes, which pays in the self attention kernel, 113.
 template <int D>
@@ -109,8 +112,8 @@ struct Fwd {
     uint64_t q_full[2];             // 8 warp arrivals
     uint64_t k_full[NS], v_full[NS];
     uint64_t k_free[NS], v_free[NS];
-    uint64_t s_full[2], s_read[2], p_full[2], o_done[2];
-    uint64_t stagger, drain[2];  // stagger: A is half way through its first step (8 warp arrivals)
+    uint64_t s_full[2], s_read[2], p_half[2], p_full[2], o_done[2];  // p_half: weights of 64 keys
+    uint64_t drain[2];
     uint32_t tmem_base;
     int abort_flag;
   };
@@ -174,10 +177,10 @@ __global__ void __launch_bounds__(Fwd<D>::THREADS, 1)
       mbar_init(&st->q_full[h], 8);
       mbar_init(&st->s_full[h], 1);
       mbar_init(&st->s_read[h], 8);
+      mbar_init(&st->p_half[h], 8);
       mbar_init(&st->p_full[h], 8);
       mbar_init(&st->o_done[h], 1);
     }
-    mbar_init(&st->stagger, 8);
     for (int i = 0; i < 2; ++i) mbar_init(&st->drain[i], 1);
     st->abort_flag = 0;
     fence_barrier_init();
@@ -241,24 +244,27 @@ __global__ void __launch_bounds__(Fwd<D>::THREADS, 1)
       issued = true;
       umma_commit_w(&st->s_full[h]);
     };
-    const auto issue_pv = [&](int h, int j) {
+    const auto issue_pv = [&](int h, int j, int part) {
       const uint64_t vd = smem_desc_sw128(smem_u32(sV(j % NS)), CH, 1024);
       const uint32_t o = tmem + F::O_COL + h * F::O_STEP, pr = tmem + F::P_COL + h * F::P_STEP;
-      umma_f16_ts4_w(o, pr, vd, IDESC_O, j > 0 ? 1u : 0u);
-      umma_f16_ts4_w(o, pr + 32, vd + (4 * 2048 >> 4), IDESC_O, 1u);
-      umma_commit_w(&st->o_done[h]);
+      umma_f16_ts4_w(o, pr + part * 32, vd + part * (4 * 2048 >> 4), IDESC_O, j > 0 || part > 0 ? 1u : 0u);
     };
     // Scores of step j (their K tile has been waited for).
     const auto scores = [&](int h, int j) {
       tc_fence_after();
       issue_s(h, j);
     };
-    // Weights of step j times V; p_full[h] next completes for P_h(j+1), which needs what is issued after this wait.
+    // Weights of step j times V, 64 keys at a time; p_half[h] and p_full[h] next complete for P_h(j+1), which needs
+    // what is issued after these waits.
     const auto sums = [&](int h, int j) {
+      if (!wait(&st->p_half[h], j & 1)) return false;
+      tc_fence_after();
+      issue_pv(h, j, 0);
+      issued = true;
       if (!wait(&st->p_full[h], j & 1)) return false;
       tc_fence_after();
-      issue_pv(h, j);
-      issued = true;
+      issue_pv(h, j, 1);
+      umma_commit_w(&st->o_done[h]);
       return true;
     };
     // V of step j, its masked rows zeroed: keys past kv_end that memory holds (TMA zero-fills past kv_len), and holes.
@@ -272,7 +278,7 @@ __global__ void __launch_bounds__(Fwd<D>::THREADS, 1)
     if (n > 0 && warp == 1) {
       for (int h = 0; h < 2 && ok; ++h) {
         if (!act[h]) continue;
-        if (F::OWN_P && h == 1 && act[0]) ok = wait(&st->stagger, 0);
+        if (F::OWN_P && h == 1 && act[0]) ok = wait(&st->p_half[0], 0);
         if (ok && (ok = wait(&st->q_full[h], 0) && wait(&st->k_full[0], 0))) scores(h, 0);
       }
       if (ok && NS < n) umma_commit_w(&st->k_free[0]);
@@ -285,7 +291,7 @@ __global__ void __launch_bounds__(Fwd<D>::THREADS, 1)
       };
       const auto next_keys = [&] { return j + 1 >= n || wait(&st->k_full[(j + 1) % NS], ((j + 1) / NS) & 1); };
       if constexpr (F::OWN_P) {
-        // Tile B is half a step behind A (see stagger): one tile's exponentials run beside the rest of the
+        // Tile B is half a step behind A (its first scores wait for A's first weights): one tile's exponentials run beside the rest of the
         // other's softmax.
         if (warp == 1) {
           if (j + 1 == n || !(ok = next_keys())) break;
@@ -340,7 +346,7 @@ __global__ void __launch_bounds__(Fwd<D>::THREADS, 1)
       const int row = quarter * 32 + lane;  // = TMEM lane
       const uint32_t lane_base = static_cast<uint32_t>(quarter * 32) << 16;
       const uint32_t s_tmem = tmem + lane_base + static_cast<uint32_t>(h * 128);
-      const uint32_t p_tmem = tmem + lane_base + F::P_COL + h * F::P_STEP + half * 32;
+      const uint32_t p_tmem = tmem + lane_base + F::P_COL + h * F::P_STEP + half * 16;
       const uint32_t o_tmem = tmem + lane_base + F::O_COL + h * F::O_STEP;
       constexpr int OC = D / 2;
       float m = -INFINITY, l = 0.0f;
@@ -371,14 +377,15 @@ __global__ void __launch_bounds__(Fwd<D>::THREADS, 1)
         return __all_sync(0xffffffffu, got) != 0;
       };
       for (int j = 0; j < n; ++j) {
-        const int kv0 = (t_lo + j) * TILE + half * 64;
-        const bool partial = mask || kv0 + 64 > kv_end;
-        if (partial) load_mask_bytes(mask, kv0, kv_end, lane, byte);
+        const int kv0 = (t_lo + j) * TILE;
+        const bool partial = mask || kv0 + TILE > kv_end;
+        if (partial) load_mask_bytes(mask, kv0 + half * 32, kv_end, lane, byte, 64);
         // s_full[h] next completes for S_h(j+1), which needs P_h(j) from these warps first.
         if (!(ok = warp_wait_ready(&st->s_full[h], j & 1, abort_flag, p.err, kErrCrossSoftmaxWait))) break;
         tc_fence_after();
-        uint32_t r[64];
-        tmem_ld64(s_tmem + half * 64, r);
+        uint32_t r[2][32];  // keys half * 32.. and 64 + half * 32..
+        tmem_ld32(s_tmem + half * 32, r[0]);
+        tmem_ld32(s_tmem + 64 + half * 32, r[1]);
         if (F::OWN_P) {
           tc_fence_before();
           __syncwarp();
@@ -390,15 +397,15 @@ __global__ void __launch_bounds__(Fwd<D>::THREADS, 1)
             const unsigned w = __ballot_sync(0xffffffffu, byte[c]);
 #pragma unroll
             for (int e = 0; e < 32; ++e)
-              if (!((w >> e) & 1u)) r[c * 32 + e] = __float_as_uint(-INFINITY);
+              if (!((w >> e) & 1u)) r[c][e] = __float_as_uint(-INFINITY);
           }
         }
         float pm[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) pm[i] = __uint_as_float(r[i]);
+        for (int i = 0; i < 8; ++i) pm[i] = __uint_as_float(r[0][i]);
 #pragma unroll
         for (int e = 8; e < 64; e += 2)
-          pm[(e >> 1) & 7] = max3(pm[(e >> 1) & 7], __uint_as_float(r[e]), __uint_as_float(r[e + 1]));
+          pm[(e >> 1) & 7] = max3(pm[(e >> 1) & 7], __uint_as_float(r[e >> 5][e & 31]), __uint_as_float(r[e >> 5][(e & 31) + 1]));
         float mx = max3(max3(pm[0], pm[1], pm[2]), max3(pm[3], pm[4], pm[5]), fmaxf(pm[6], pm[7])), mo;
         if (!(ok = swap(static_cast<uint32_t>(j), mx, &mo))) break;
         mx = fmaxf(mx, mo) * p.scale_log2;
@@ -437,25 +444,21 @@ __global__ void __launch_bounds__(Fwd<D>::THREADS, 1)
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
             float x0, x1, e0, e1;
-            unpk2(fma2(pk2(__uint_as_float(r[g * 32 + 2 * i]), __uint_as_float(r[g * 32 + 2 * i + 1])), sc2, nm2), x0, x1);
+            unpk2(fma2(pk2(__uint_as_float(r[g][2 * i]), __uint_as_float(r[g][2 * i + 1])), sc2, nm2), x0, x1);
             e0 = fast_exp2(x0);
             e1 = fast_exp2(x1);
             ps2[i & 3] = add2(ps2[i & 3], pk2(e0, e1));
             w[i] = pack_bf16x2(e0, e1);
           }
-          tmem_st16(p_tmem + g * 16, w);
-          if (F::OWN_P && g == 0 && j == 0 && h == 0) {
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&st->stagger);
-          }
+          tmem_st16(p_tmem + g * 32, w);
+          tmem_wait_st();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(g == 0 ? &st->p_half[h] : &st->p_full[h]);
         }
         float x, y;
         unpk2(add2(add2(ps2[0], ps2[1]), add2(ps2[2], ps2[3])), x, y);
         l += x + y;
-        tmem_wait_st();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&st->p_full[h]);
       }
       if (ok && n > 0)
         ok = warp_wait_ready(&st->o_done[h], (n - 1) & 1, abort_flag, p.err, kErrCrossSoftmaxWait);
