@@ -504,7 +504,7 @@ __global__ void __launch_bounds__(FWD_THREADS, 1)
 //   warp 1  MMA: S, dP, then the sums with P and dS (hi and lo) from TMEM; the next tile's S and dP run while the
 //           sums are folded
 //   warps 2..9  X into TMEM, then two warps to a row: P, dS, and a tile's sums folded into registers
-// The tensor pipe bounds it: 3072 cycles a tile of 64 rows for dk and dv at D = 64, 2304 for dq.
+// The tensor pipe bounds it: 96 steps of 32 cycles a tile of 64 rows for dk and dv at D = 64, 72 for dq.
 // B200, [4, 16, 333 x 1000, 64]: 258 us, planes included (782 on the CUDA cores), D = 128: 608 (1852); one row a pair
 // 123 (226); [2, 8, 77 x 300, 64] 29 (84).
 enum GradPass { kGradDq, kGradDkv, kGradDk, kGradDv };
