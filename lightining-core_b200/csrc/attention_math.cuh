@@ -73,11 +73,4 @@ __device__ __forceinline__ float tf32_round(float x) {
   return __uint_as_float(u);
 }
 
-// 2^x, MUFU ex2 without flush-to-zero (relative error ~2^-22).
-__device__ __forceinline__ float exp2_acc(float x) {
-  float y;
-  asm("ex2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
 }  // namespace lcb

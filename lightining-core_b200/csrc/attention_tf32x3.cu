@@ -89,6 +89,13 @@ struct Params {
   unsigned* err_word;
 };
 
+// 2^x, MUFU ex2 without flush-to-zero (relative error ~2^-22).
+__device__ __forceinline__ float exp2_acc(float x) {
+  float y;
+  asm("ex2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
 // ---- pre-pass -----------------------------------------------------------------------------------
 // Rows of 64 floats (unit u at src + u*unit_stride) -> contiguous hi/lo planes [units, S, 64],
 // by `nblk` blocks of 256 threads (block `bx`), four floats per thread when the unit start is

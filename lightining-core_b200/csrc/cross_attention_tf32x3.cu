@@ -233,7 +233,7 @@ __device__ __forceinline__ void store_cols(float* out, const float* v, float f, 
 //               tagged shared-memory words and P_hi lies over S_j's columns; at D = 128 a tile has 32 keys, each
 //               warp reads them all and P_hi has columns of its own.
 // The tensor pipe bounds it: 1536 cycles a tile of 64 keys at D = 64.
-// B200, [4, 16, 333 x 1000, 64] with holes: 90 us, planes included (370 us on the CUDA cores); D = 128: 181 (698).
+// B200, [4, 16, 333 x 1000, 64] with holes: 84 us, planes included (370 us on the CUDA cores); D = 128: 174 (698).
 template <int D>
 struct Fwd {
   static constexpr int T = 4096 / D, VS = D == 64 ? 2 : 1, OC = D / 2;
@@ -333,7 +333,7 @@ __global__ void __launch_bounds__(FWD_THREADS, 1)
   } else if (warp == 1) {
     // ------------------------------------------------------------ MMA (whole warp)
     bool ok = n > 0, issued = false;
-    const auto wait = [&](uint64_t* bar, uint32_t ph) { return warp_wait_poll(bar, ph, abort_flag, err, kErrCrossMmaWait); };
+    const auto wait = [&](uint64_t* bar, uint32_t ph) { return warp_wait_ready(bar, ph, abort_flag, err, kErrCrossMmaWait); };
     const auto issue_s = [&](int j) {
       if (!wait(&st->k_full[j & 1], (j >> 1) & 1)) return false;
       tc_fence_after();
@@ -389,7 +389,7 @@ __global__ void __launch_bounds__(FWD_THREADS, 1)
       return true;
     };
     const auto fold = [&](int t, float alpha) {
-      if (!warp_wait_poll(&st->o_full[t & 1], (t >> 1) & 1, abort_flag, err, kErrCrossSoftmaxWait)) return false;
+      if (!warp_wait_ready(&st->o_full[t & 1], (t >> 1) & 1, abort_flag, err, kErrCrossSoftmaxWait)) return false;
       tc_fence_after();
 #pragma unroll
       for (int c = 0; c < OC; c += 32) {
@@ -408,7 +408,7 @@ __global__ void __launch_bounds__(FWD_THREADS, 1)
       const bool partial = mask || kv0 + 32 > kv_end;
       bool seen = true;
       if (partial) seen = kv0 + lane < kv_end && (!mask || mask[kv0 + lane]);
-      if (!(ok = warp_wait_poll(&st->s_full[s], (j >> 1) & 1, abort_flag, err, kErrCrossSoftmaxWait))) break;
+      if (!(ok = warp_wait_ready(&st->s_full[s], (j >> 1) & 1, abort_flag, err, kErrCrossSoftmaxWait))) break;
       tc_fence_after();
       uint32_t r[32];
       tmem_ld32(lanes + F::S_COL + static_cast<uint32_t>(s * T + own), r);
@@ -444,7 +444,7 @@ __global__ void __launch_bounds__(FWD_THREADS, 1)
       float p[32], ls4[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
       for (int e = 0; e < 32; ++e) {
-        p[e] = exp2_acc(__fmaf_rn(__uint_as_float(r[e]), scale_log2, -mu));
+        p[e] = fast_exp2(__fmaf_rn(__uint_as_float(r[e]), scale_log2, -mu));
         ls4[e & 3] += p[e];
       }
       l += (ls4[0] + ls4[1]) + (ls4[2] + ls4[3]);
@@ -505,8 +505,8 @@ __global__ void __launch_bounds__(FWD_THREADS, 1)
 //           sums are folded
 //   warps 2..9  X into TMEM, then two warps to a row: P, dS, and a tile's sums folded into registers
 // The tensor pipe bounds it: 96 steps of 32 cycles a tile of 64 rows for dk and dv at D = 64, 72 for dq.
-// B200, [4, 16, 333 x 1000, 64]: 258 us, planes included (782 on the CUDA cores), D = 128: 608 (1852); one row a pair
-// 123 (226); [2, 8, 77 x 300, 64] 29 (84).
+// B200, [4, 16, 333 x 1000, 64]: 232 us, planes included (782 on the CUDA cores), D = 128: 562 (1852); one row a pair
+// 123 (226); [2, 8, 77 x 300, 64] 27 (84).
 enum GradPass { kGradDq, kGradDkv, kGradDk, kGradDv };
 
 template <int D>
@@ -649,7 +649,7 @@ __global__ void __launch_bounds__(GRAD_THREADS, 1) cross_grad_f32_tc_kernel(cons
     }
   } else if (warp == 1) {
     // ------------------------------------------------------------ MMA (whole warp)
-    const auto wait = [&](uint64_t* bar, uint32_t ph) { return warp_wait_poll(bar, ph, abort_flag, p.err, kErrCrossMmaWait); };
+    const auto wait = [&](uint64_t* bar, uint32_t ph) { return warp_wait_ready(bar, ph, abort_flag, p.err, kErrCrossMmaWait); };
     bool issued = false, ok = n > 0;
     int i = 0;
     const auto piece = [&] { return wait(&st->full[i % NP], (i / NP) & 1); };
@@ -696,7 +696,7 @@ __global__ void __launch_bounds__(GRAD_THREADS, 1) cross_grad_f32_tc_kernel(cons
     const int quarter = warp & 3, half = warp >= 6 ? 1 : 0;
     const int row = quarter * 32 + lane, r = r0 + row;
     const uint32_t lanes = tmem + (static_cast<uint32_t>(quarter * 32) << 16), hc = static_cast<uint32_t>(half * SC);
-    const auto wait = [&](uint64_t* bar, uint32_t ph) { return warp_wait_poll(bar, ph, abort_flag, p.err, kErrCrossSoftmaxWait); };
+    const auto wait = [&](uint64_t* bar, uint32_t ph) { return warp_wait_ready(bar, ph, abort_flag, p.err, kErrCrossSoftmaxWait); };
     const auto arrive = [&](uint64_t* bar) {
       tc_fence_before();
       __syncwarp();
@@ -745,7 +745,7 @@ __global__ void __launch_bounds__(GRAD_THREADS, 1) cross_grad_f32_tc_kernel(cons
       const float2* tm = st->terms[ph] + half * SC;
 #pragma unroll
       for (int e = 0; e < SC; ++e) {
-        const float x = exp2_acc(__fmaf_rn(__uint_as_float(w[e]), p.scale_log2, keys ? tm[e].x : mine.x));
+        const float x = fast_exp2(__fmaf_rn(__uint_as_float(w[e]), p.scale_log2, keys ? tm[e].x : mine.x));
         pr[e] = (keys ? seen : ((vis >> e) & 1u) != 0) ? x : 0.0f;
       }
       if (with_p) {
