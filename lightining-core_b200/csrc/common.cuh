@@ -510,6 +510,37 @@ __device__ __forceinline__ void umma_f16_ts4k_w(uint32_t d_tmem, uint32_t a_tmem
       "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
       : "memory");
 }
+// The same for tf32 (8 values = 32 bytes on per step): both operands in shared memory, or A in TMEM (8 columns on).
+__device__ __forceinline__ void umma_tf32_ss4_w(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                                uint32_t accumulate) {
+  asm volatile(
+      "{\n .reg .pred p, t, e;\n .reg .b64 a1, b1, a2, b2, a3, b3;\n"
+      " setp.ne.b32 p, %4, 0;\n setp.eq.b32 t, 0, 0;\n"
+      " add.s64 a1, %1, 2;\n add.s64 b1, %2, 2;\n add.s64 a2, %1, 4;\n add.s64 b2, %2, 4;\n"
+      " add.s64 a3, %1, 6;\n add.s64 b3, %2, 6;\n"
+      " elect.sync _|e, 0xffffffff;\n"
+      " @e tcgen05.mma.cta_group::1.kind::tf32 [%0], %1, %2, %3, p;\n"
+      " @e tcgen05.mma.cta_group::1.kind::tf32 [%0], a1, b1, %3, t;\n"
+      " @e tcgen05.mma.cta_group::1.kind::tf32 [%0], a2, b2, %3, t;\n"
+      " @e tcgen05.mma.cta_group::1.kind::tf32 [%0], a3, b3, %3, t;\n}\n" ::"r"(d_tmem),
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void umma_tf32_ts4k_w(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc,
+                                                 uint32_t accumulate) {
+  asm volatile(
+      "{\n .reg .pred p, t, e;\n .reg .b32 a1, a2, a3;\n .reg .b64 b1, b2, b3;\n"
+      " setp.ne.b32 p, %4, 0;\n setp.eq.b32 t, 0, 0;\n"
+      " add.s32 a1, %1, 8;\n add.s32 a2, %1, 16;\n add.s32 a3, %1, 24;\n"
+      " add.s64 b1, %2, 2;\n add.s64 b2, %2, 4;\n add.s64 b3, %2, 6;\n"
+      " elect.sync _|e, 0xffffffff;\n"
+      " @e tcgen05.mma.cta_group::1.kind::tf32 [%0], [%1], %2, %3, p;\n"
+      " @e tcgen05.mma.cta_group::1.kind::tf32 [%0], [a1], b1, %3, t;\n"
+      " @e tcgen05.mma.cta_group::1.kind::tf32 [%0], [a2], b2, %3, t;\n"
+      " @e tcgen05.mma.cta_group::1.kind::tf32 [%0], [a3], b3, %3, t;\n}\n" ::"r"(d_tmem),
+      "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
 // Warp-uniform bounded wait: lane 0 waits, the result is broadcast.
 __device__ __forceinline__ bool warp_wait_bounded(uint64_t* bar, uint32_t parity, volatile int* abort_flag,
                                                   unsigned* err, unsigned code) {

@@ -153,17 +153,15 @@ __device__ __forceinline__ void mma_scores(uint32_t d, const uint8_t* a, const u
   constexpr uint32_t IDESC = idesc_tf32_f32(TILE, T, 0, 0);
   const uint64_t ah = smem_desc_sw128(smem_u32(a), 16, 1024), al = smem_desc_sw128(smem_u32(a + D / 32 * ACH), 16, 1024);
   const uint64_t bh = smem_desc_sw128(smem_u32(piece), 16, 1024), bl = smem_desc_sw128(smem_u32(piece + PIECE / 2), 16, 1024);
+  // (Chunks of 32 values, four steps each.)
 #pragma unroll
-  for (int k = 0; k < D / 8; ++k) {
-    const uint32_t ao = ((k >> 2) * ACH + (k & 3) * 32) >> 4, bo = ((k >> 2) * T * 128 + (k & 3) * 32) >> 4;
-    umma_tf32_ss_w(d, al + ao, bh + bo, IDESC, k > 0 ? 1u : 0u);
-    umma_tf32_ss_w(d, ah + ao, bl + bo, IDESC, 1u);
+  for (int c = 0; c < D / 32; ++c) {
+    const uint32_t ao = c * ACH >> 4, bo = c * T * 128 >> 4;
+    umma_tf32_ss4_w(d, al + ao, bh + bo, IDESC, c > 0 ? 1u : 0u);
+    umma_tf32_ss4_w(d, ah + ao, bl + bo, IDESC, 1u);
   }
 #pragma unroll
-  for (int k = 0; k < D / 8; ++k) {
-    const uint32_t ao = ((k >> 2) * ACH + (k & 3) * 32) >> 4, bo = ((k >> 2) * T * 128 + (k & 3) * 32) >> 4;
-    umma_tf32_ss_w(d, ah + ao, bh + bo, IDESC, 1u);
-  }
+  for (int c = 0; c < D / 32; ++c) umma_tf32_ss4_w(d, ah + (c * ACH >> 4), bh + (c * T * 128 >> 4), IDESC, 1u);
 }
 // d[128 x N] = A[128 x K] . piece[N x K]^T, A's hi and lo columns in TMEM.
 template <int N, int K>
@@ -171,16 +169,12 @@ __device__ __forceinline__ void mma_tmem(uint32_t d, uint32_t ah, uint32_t al, c
   constexpr uint32_t IDESC = idesc_tf32_f32(TILE, N, 0, 0);
   const uint64_t bh = smem_desc_sw128(smem_u32(piece), 16, 1024), bl = smem_desc_sw128(smem_u32(piece + PIECE / 2), 16, 1024);
 #pragma unroll
-  for (int k = 0; k < K / 8; ++k) {
-    const uint32_t bo = ((k >> 2) * N * 128 + (k & 3) * 32) >> 4;
-    umma_tf32_ts_w(d, al + k * 8, bh + bo, IDESC, k > 0 ? 1u : 0u);
-    umma_tf32_ts_w(d, ah + k * 8, bl + bo, IDESC, 1u);
+  for (int c = 0; c < K / 32; ++c) {
+    umma_tf32_ts4k_w(d, al + c * 32, bh + (c * N * 128 >> 4), IDESC, c > 0 ? 1u : 0u);
+    umma_tf32_ts4k_w(d, ah + c * 32, bl + (c * N * 128 >> 4), IDESC, 1u);
   }
 #pragma unroll
-  for (int k = 0; k < K / 8; ++k) {
-    const uint32_t bo = ((k >> 2) * N * 128 + (k & 3) * 32) >> 4;
-    umma_tf32_ts_w(d, ah + k * 8, bh + bo, IDESC, 1u);
-  }
+  for (int c = 0; c < K / 32; ++c) umma_tf32_ts4k_w(d, ah + c * 32, bh + (c * N * 128 >> 4), IDESC, 1u);
 }
 template <int N>
 __device__ __forceinline__ void tmem_read(uint32_t at, uint32_t (&r)[N]) {
