@@ -166,6 +166,7 @@ __device__ __forceinline__ void store_rows(T* out, const float (&o)[4][Tile<DP, 
 template <typename T, int DP, int TT>
 __global__ void __launch_bounds__(Tile<DP, TT>::NT) cross_fwd_simt_kernel(CrossArgs a, CrossSplit sp, int vec) {
   using L = Tile<DP, TT>;
+  griddep_launch_dependents();  // the parts' join waits for the end of this grid
   extern __shared__ __align__(16) float smem[];
   float *Q = smem, *K = Q + L::ROWS, *V = K + L::ROWS, *P = V + L::ROWS;
   __shared__ unsigned char seen[TT];
@@ -314,7 +315,8 @@ __global__ void __launch_bounds__(256) cross_combine_kernel(CrossArgs a, CrossSp
 // Row terms, negated so that they are addends: -D with D = dout . out, and minus the row's
 // log-sum-exp in the log2 domain.  Rows that are not computed or see no key get -infinity and 0:
 // every weight exp2(s - inf) is 0.  One warp to a row; rows of the workspace are padded to whole
-// tiles of 128 tokens.
+// tiles of 128 tokens.  (The walks' blocks do not come in beside these kernels' last ones: they took 8 us from
+// them that way.)
 template <typename T>
 __global__ void __launch_bounds__(256) cross_row_terms_kernel(CrossGradArgs g, float* neg_lse2, float* neg_d, int q_pad,
                                                               long long rows) {
@@ -706,11 +708,8 @@ cudaError_t CrossSplitWork::end(const CrossArgs& a, cudaError_t e, cudaStream_t 
   if (sp.splits <= 1) return e;
   if (e == cudaSuccess) {
     const long long blocks = (sp.rows + 7) / 8;
-    if (a.bf16)
-      cross_combine_kernel<__nv_bfloat16><<<static_cast<unsigned>(blocks), 256, 0, s>>>(a, sp);
-    else
-      cross_combine_kernel<float><<<static_cast<unsigned>(blocks), 256, 0, s>>>(a, sp);
-    e = cudaGetLastError();
+    const auto kernel = a.bf16 ? cross_combine_kernel<__nv_bfloat16> : cross_combine_kernel<float>;
+    e = launch_pdl(kernel, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, s, a, sp);
   }
   const cudaError_t f = workspace_free(ws, s);
   return e != cudaSuccess ? e : f;

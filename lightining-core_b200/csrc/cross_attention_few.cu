@@ -223,6 +223,7 @@ __global__ void __launch_bounds__(THREADS, 2)
     return;
   }
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
+  griddep_launch_dependents();  // the parts' join waits for the end of this grid
   const FewJob<L> job(a, sp, cluster);
   if (threadIdx.x == 0) few_init<L>(bars, &map_k, &map_v);
   __syncthreads();
@@ -379,6 +380,7 @@ __global__ void __launch_bounds__(THREADS, 2)
     return;
   }
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
+  griddep_launch_dependents();  // the parts' join waits for the end of this grid
   const FewJob<L> job(a, sp, cluster);
   if (threadIdx.x == 0) few_init<L>(bars, &map_k, &map_v);
   for (int i = threadIdx.x; i < R * D / 4; i += THREADS) {

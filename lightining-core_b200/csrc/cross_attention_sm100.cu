@@ -143,6 +143,7 @@ __global__ void __launch_bounds__(Fwd<D>::THREADS, 1)
   const auto sQ = [&](int h) { return smem + h * F::BYTES; };
   const auto sK = [&](int s) { return smem + F::K_OFF + s * F::BYTES; };
   const auto sV = [&](int s) { return smem + F::V_OFF + s * F::BYTES; };
+  griddep_launch_dependents();  // the parts' join waits for the end of this grid
   const CrossArgs& a = p.a;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
@@ -544,8 +545,8 @@ __global__ void __launch_bounds__(Fwd<D>::THREADS, 1)
 //   * three issuing warps, for S, dP and the sums, which order each other by barriers only
 //   * resident blocks that go from job to job: four more warps load the next job's rows and store
 //     the last one's sums meanwhile (two sets of TMEM columns where they fit)
-// B200, row terms included: [16, 16, 512 x 2048 ragged, 64] 306 us (blocks of one job with one chain of products:
-// 471), [4, 16/4, 1024 x 2048 ragged, 128] 227 us (266).
+// B200, row terms included: [16, 16, 512 x 2048 ragged, 64] 270 us (blocks of one job with one chain of products:
+// 471), [4, 16/4, 1024 x 2048 ragged, 128] 188 us (266).
 constexpr int QT = 64;         // rows of an item
 constexpr int QCH = QT * 128;  // one [64 rows x 64 bf16] box
 template <int D, bool KV>
@@ -590,6 +591,7 @@ struct GradParams {
   int y1_head, y1_batch, y2_head, y2_batch;  // 1: the map of the streamed tensor has that axis
   int x1_head, x1_batch, x2_head, x2_batch;  // KV: the same of k and v, and of their gradients
   int jobs, tiles;                           // tiles of rows of a (batch, key head) pair
+  int beside;                                // the dq walk may run beside the other
   float scale_log2;
   unsigned* err;
 };
@@ -687,6 +689,10 @@ __global__ void __launch_bounds__(Grad<D, KV>::THREADS, 1)
   const uint32_t tmem = st->tmem_base;
   volatile int* abort_flag = &st->abort_flag;
   const int grid = static_cast<int>(gridDim.x);
+  // The row terms, and whatever ran before.  The dq walk may start once every block of the other one has passed
+  // here, and takes the SMs that its last jobs leave idle; it is not over before the other is (see the end).
+  if (KV || !p.beside) griddep_wait();
+  if (KV) griddep_launch_dependents();
   // Every role counts the items it has passed (i) and the jobs that have some (x); item i belongs to group
   // i & 1 and stage i % NS, job x to columns x % NX and x % NA.  Each barrier's next completion needs
   // what its waiters do after this one, so no parity wait is ambiguous.
@@ -1148,6 +1154,7 @@ __global__ void __launch_bounds__(Grad<D, KV>::THREADS, 1)
     tc_fence_after();
     tmem_dealloc(tmem, 512);
   }
+  if (!KV) griddep_wait();
 }
 
 // ---- host -------------------------------------------------------------------------------------
@@ -1213,7 +1220,9 @@ cudaError_t bwd_tc(const CrossGradArgs& g, const float* neg_lse2, const float* n
   const CrossArgs& a = g.f;
   DeviceCtx* ctx = device_ctx();
   if (!ctx) return cudaErrorNoDevice;
-  // One walk: resident blocks, one to an SM.
+  // One walk: resident blocks, one to an SM.  (The dq walk beside the other's last jobs: [4, 16/4, 1024 x 2048 ragged,
+  // 128] 188 us, one after the other 210; with two or four blocks to an SM, dealt out as they get free, 191 and
+  // 197.)
   const auto walk = [&](auto kv, const HeadMap& y1, const HeadMap& y2, const HeadMap& x1, const HeadMap& x2,
                         const HeadMap& dk, const HeadMap& dv, int tiles, int entries) -> cudaError_t {
     constexpr bool KV = decltype(kv)::value;
@@ -1225,10 +1234,10 @@ cudaError_t bwd_tc(const CrossGradArgs& g, const float* neg_lse2, const float* n
     if (jobs > 0x7fffffffLL - ctx->sm_count) return cudaErrorNotSupported;
     const GradParams p{g,           neg_lse2,   neg_d,       q_pad,      y1.by_head,  y1.by_batch,
                        y2.by_head,  y2.by_batch, x1.by_head, x1.by_batch, x2.by_head, x2.by_batch,
-                       static_cast<int>(jobs), tiles, a.scale * kLog2e, ctx->err_word};
+                       static_cast<int>(jobs), tiles, !KV && g.dk, a.scale * kLog2e, ctx->err_word};
     const unsigned blocks = static_cast<unsigned>(std::min<long long>(jobs, ctx->sm_count));
-    cross_grad_tc_kernel<D, KV><<<blocks, L::THREADS, L::SMEM, s>>>(y1.map, y2.map, x1.map, x2.map, dk.map, dv.map, p);
-    return cudaGetLastError();
+    return launch_pdl(cross_grad_tc_kernel<D, KV>, dim3(blocks), dim3(L::THREADS), L::SMEM, s, y1.map, y2.map, x1.map, x2.map,
+                      dk.map, dv.map, p);
   };
   HeadMap m1, m2, x1{}, x2{}, dk{}, dv{};
   if (g.dk) {

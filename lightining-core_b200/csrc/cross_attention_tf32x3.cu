@@ -253,6 +253,7 @@ __global__ void __launch_bounds__(FWD_THREADS, 1)
                         float scale_log2, int vec_out, unsigned* err) {
   using F = Fwd<D>;
   constexpr int T = F::T, OC = F::OC;
+  griddep_launch_dependents();  // the parts' join waits for the end of this grid
   extern __shared__ __align__(16) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   typename F::Tail* st = reinterpret_cast<typename F::Tail*>(smem + F::TAIL_OFF);
