@@ -545,8 +545,8 @@ __global__ void __launch_bounds__(Fwd<D>::THREADS, 1)
 //   * three issuing warps, for S, dP and the sums, which order each other by barriers only
 //   * resident blocks that go from job to job: four more warps load the next job's rows and store
 //     the last one's sums meanwhile (two sets of TMEM columns where they fit)
-// B200, row terms included: [16, 16, 512 x 2048 ragged, 64] 270 us (blocks of one job with one chain of products:
-// 471), [4, 16/4, 1024 x 2048 ragged, 128] 188 us (266).
+// B200, row terms included: [16, 16, 512 x 2048 ragged, 64] 267 us (blocks of one job with one chain of products:
+// 471), [4, 16/4, 1024 x 2048 ragged, 128] 185 us (266).
 constexpr int QT = 64;         // rows of an item
 constexpr int QCH = QT * 128;  // one [64 rows x 64 bf16] box
 template <int D, bool KV>
@@ -591,6 +591,7 @@ struct GradParams {
   int y1_head, y1_batch, y2_head, y2_batch;  // 1: the map of the streamed tensor has that axis
   int x1_head, x1_batch, x2_head, x2_batch;  // KV: the same of k and v, and of their gradients
   int jobs, tiles;                           // tiles of rows of a (batch, key head) pair
+  int group, step_tile, step_hk, step_b;     // rows' heads to a key head; the grid's size in jobs' digits
   int beside;                                // the dq walk may run beside the other
   float scale_log2;
   unsigned* err;
@@ -598,30 +599,41 @@ struct GradParams {
 
 // A job's rows.  Its items are, in order: the batch entries [b, b_hi) with span() > 0, `heads` heads each, tiles
 // of 64 rows up to span().
+// A block goes from job to job by adding the grid's size in (batch entry, key head, tile) digits (with divisions
+// 270 and 188 us where it is 267 and 185).
 template <bool KV>
 struct Job {
-  int b, hk, r0, b_hi, group, heads;
-  __device__ Job(const GradParams& p, int job) {
-    const CrossArgs& a = p.g.f;
-    const int pair = job / p.tiles;
-    b = pair / a.hk;
-    hk = pair % a.hk;
-    r0 = (job % p.tiles) * TILE;
-    b_hi = KV && p.g.kv_shared ? a.batch : b + 1;
-    group = a.hq / a.hk;
-    heads = KV ? group : 1;
+  int job, b, hk, tile;
+  __device__ explicit Job(const GradParams& p) {
+    job = blockIdx.x;
+    tile = job % p.tiles;
+    hk = job / p.tiles % p.g.f.hk;
+    b = job / p.tiles / p.g.f.hk;
   }
+  __device__ void step(const GradParams& p) {
+    job += gridDim.x;
+    tile += p.step_tile;
+    hk += p.step_hk;
+    b += p.step_b;
+    if (tile >= p.tiles) tile -= p.tiles, ++hk;
+    if (hk >= p.g.f.hk) hk -= p.g.f.hk, ++b;
+  }
+  __device__ int r0() const { return tile * TILE; }
+  __device__ int b_hi(const GradParams& p) const { return KV && p.g.kv_shared ? p.g.f.batch : b + 1; }
+  __device__ int heads(const GradParams& p) const { return KV ? p.group : 1; }
   // Rows of batch entry yb to walk (0: none), for KV the queries if the tile has a key to see, else the keys if
   // the tile has a query to compute: its first row's token is one, or another head starts in it.
-  __device__ int span(const CrossArgs& a, int yb) const {
+  __device__ int span(const GradParams& p, int yb) const {
+    const CrossArgs& a = p.g.f;
     const int q_end = cross_len(a.q_lens, yb, a.q_len), kv_end = cross_len(a.kv_lens, yb, a.kv_len);
-    if (KV) return r0 < kv_end ? q_end : 0;
-    const int t = r0 % a.q_len;
-    return q_end > 0 && (t < q_end || r0 + a.q_len - t < min(r0 + TILE, group * a.q_len)) ? kv_end : 0;
+    if (KV) return r0() < kv_end ? q_end : 0;
+    if (q_end == a.q_len) return kv_end;
+    const int t = r0() % a.q_len;
+    return q_end > 0 && (t < q_end || r0() + a.q_len - t < min(r0() + TILE, p.group * a.q_len)) ? kv_end : 0;
   }
-  __device__ int count(const CrossArgs& a) const {
+  __device__ int count(const GradParams& p) const {
     int n = 0;
-    for (int yb = b; yb < b_hi; ++yb) n += heads * ((span(a, yb) + QT - 1) / QT);
+    for (int yb = b; yb < b_hi(p); ++yb) n += heads(p) * ((span(p, yb) + QT - 1) / QT);
     return n;
   }
 };
@@ -688,7 +700,6 @@ __global__ void __launch_bounds__(Grad<D, KV>::THREADS, 1)
   tc_fence_after();
   const uint32_t tmem = st->tmem_base;
   volatile int* abort_flag = &st->abort_flag;
-  const int grid = static_cast<int>(gridDim.x);
   // The row terms, and whatever ran before.  The dq walk may start once every block of the other one has passed
   // here, and takes the SMs that its last jobs leave idle; it is not over before the other is (see the end).
   if (KV || !p.beside) griddep_wait();
@@ -701,16 +712,15 @@ __global__ void __launch_bounds__(Grad<D, KV>::THREADS, 1)
     // ------------------------------------------------------------ TMA producer
     bool ok = true;
     int i = 0, x = 0;
-    for (int job = blockIdx.x; job < p.jobs && ok; job += grid) {
-      const Job<KV> j(p, job);
+    for (Job<KV> j(p); j.job < p.jobs && ok; j.step(p)) {
       if (KV) {
-        if (j.count(a) == 0) {
+        if (j.count(p) == 0) {
           // No query sees a key of this tile: zeros, a row's pieces to neighbouring lanes.
           const int vecs = a.d / 8;
           __nv_bfloat16* dk = static_cast<__nv_bfloat16*>(p.g.dk) + j.b * a.ks.b + j.hk * a.ks.h;
           __nv_bfloat16* dv = static_cast<__nv_bfloat16*>(p.g.dv) + j.b * a.vs.b + j.hk * a.vs.h;
           for (int k = lane; k < TILE * vecs; k += 32) {
-            const int key = j.r0 + k / vecs, c = k % vecs * 8;
+            const int key = j.r0() + k / vecs, c = k % vecs * 8;
             if (key >= a.kv_len) break;
             *reinterpret_cast<uint4*>(dk + key * a.ks.t + c) = make_uint4(0, 0, 0, 0);
             *reinterpret_cast<uint4*>(dv + key * a.vs.t + c) = make_uint4(0, 0, 0, 0);
@@ -726,16 +736,16 @@ __global__ void __launch_bounds__(Grad<D, KV>::THREADS, 1)
           if (ok) {
             uint8_t* box = smem + (L::X_SMEM ? L::X_OFF : L::IN_OFF);
             mbar_arrive_expect_tx(bar, 2 * L::NCH * CH);
-            load_tile(box, &map_x1, L::NCH, j.r0, p.x1_head ? j.hk : 0, p.x1_batch ? j.b : 0, bar);
-            load_tile(box + L::NCH * CH, &map_x2, L::NCH, j.r0, p.x2_head ? j.hk : 0, p.x2_batch ? j.b : 0, bar);
+            load_tile(box, &map_x1, L::NCH, j.r0(), p.x1_head ? j.hk : 0, p.x1_batch ? j.b : 0, bar);
+            load_tile(box + L::NCH * CH, &map_x2, L::NCH, j.r0(), p.x2_head ? j.hk : 0, p.x2_batch ? j.b : 0, bar);
           }
         }
         ++x;
       }
       if (lane == 0)
-        for (int yb = j.b; yb < j.b_hi && ok; ++yb) {
-          const int y_end = j.span(a, yb);
-          for (int g = 0; g < j.heads && ok; ++g)
+        for (int yb = j.b; yb < j.b_hi(p) && ok; ++yb) {
+          const int y_end = j.span(p, yb);
+          for (int g = 0; g < j.heads(p) && ok; ++g)
             for (int t0 = 0; t0 < y_end; t0 += QT, ++i) {
               const int s = i % NS;
               if (i >= NS &&
@@ -743,7 +753,7 @@ __global__ void __launch_bounds__(Grad<D, KV>::THREADS, 1)
                 ok = false;
                 break;
               }
-              const int h = KV ? j.hk * j.group + g : j.hk;
+              const int h = KV ? j.hk * p.group + g : j.hk;
               mbar_arrive_expect_tx(&st->full[s], L::STAGE + (KV ? 512 : 0));
               for (int c = 0; c < L::NCH; ++c)
                 tma_load_4d(sY1(s) + c * QCH, &map_y1, c * 64, t0, p.y1_head ? h : 0, p.y1_batch ? yb : 0, &st->full[s]);
@@ -773,14 +783,13 @@ __global__ void __launch_bounds__(Grad<D, KV>::THREADS, 1)
       return warp_wait_ready(bar, ph, abort_flag, p.err, kErrCrossMmaWait);
     };
     int i = 0, x = 0;
-    for (int job = blockIdx.x; job < p.jobs && ok; job += grid) {
-      const Job<KV> j(p, job);
+    for (Job<KV> j(p); j.job < p.jobs && ok; j.step(p)) {
       const uint32_t rows = tmem + L::X + (x % NX) * L::XW + which * (D / 2);
       bool first = true;
-      for (int yb = j.b; yb < j.b_hi && ok; ++yb) {
-        const int y_end = j.span(a, yb), y_len = KV ? a.q_len : a.kv_len;
+      for (int yb = j.b; yb < j.b_hi(p) && ok; ++yb) {
+        const int y_end = j.span(p, yb), y_len = KV ? a.q_len : a.kv_len;
         const unsigned char* mask = !KV && a.key_mask ? a.key_mask + static_cast<long long>(yb) * a.kv_len : nullptr;
-        for (int g = 0; g < j.heads && ok; ++g)
+        for (int g = 0; g < j.heads(p) && ok; ++g)
           for (int t0 = 0; t0 < y_end; t0 += QT, ++i) {
             const int s = i % NS;
             uint8_t* y = which ? sY2(s) : sY1(s);
@@ -818,8 +827,8 @@ __global__ void __launch_bounds__(Grad<D, KV>::THREADS, 1)
       return warp_wait_ready(bar, ph, abort_flag, p.err, kErrCrossMmaWait);
     };
     int i = 0, x = 0;
-    for (int job = blockIdx.x; job < p.jobs && ok; job += grid) {
-      const int n = Job<KV>(p, job).count(a);
+    for (Job<KV> j(p); j.job < p.jobs && ok; j.step(p)) {
+      const int n = j.count(p);
       if (n == 0) continue;
       const uint32_t sums = tmem + L::A + (x % NA) * L::AW;
       if (x >= NA && !(ok = wait(&st->sums_free[x % NA], (x / NA - 1) & 1))) break;
@@ -851,23 +860,22 @@ __global__ void __launch_bounds__(Grad<D, KV>::THREADS, 1)
     const uint64_t sc2 = pk2(p.scale_log2, p.scale_log2);
     bool ok = true;
     int i0 = 0;  // items passed before this batch entry
-    for (int job = blockIdx.x; job < p.jobs && ok; job += grid) {
-      const Job<KV> j(p, job);
+    for (Job<KV> j(p); j.job < p.jobs && ok; j.step(p)) {
       uint64_t nl2 = 0, nd2 = 0;
       if (!KV) {
-        const int rr = j.r0 + row, t = rr % a.q_len;
-        const bool in = rr < j.group * a.q_len && t < cross_len(a.q_lens, j.b, a.q_len);
-        const long long term = (static_cast<long long>(j.b) * a.hq + j.hk * j.group + rr / a.q_len) * p.q_pad + t;
+        const int rr = j.r0() + row, t = rr % a.q_len;
+        const bool in = rr < p.group * a.q_len && t < cross_len(a.q_lens, j.b, a.q_len);
+        const long long term = (static_cast<long long>(j.b) * a.hq + j.hk * p.group + rr / a.q_len) * p.q_pad + t;
         const float nl = in ? p.neg_lse2[term] : -INFINITY, nd = in ? p.neg_d[term] : 0.0f;
         nl2 = pk2(nl, nl);
         nd2 = pk2(nd, nd);
       }
-      for (int yb = j.b; yb < j.b_hi && ok; ++yb) {
-        const int y_end = j.span(a, yb), n = j.heads * ((y_end + QT - 1) / QT);
+      for (int yb = j.b; yb < j.b_hi(p) && ok; ++yb) {
+        const int y_end = j.span(p, yb), n = j.heads(p) * ((y_end + QT - 1) / QT);
         const unsigned char* mask = a.key_mask ? a.key_mask + static_cast<long long>(yb) * a.kv_len : nullptr;
         bool zero = false;  // KV: this row's key is masked
         if (KV && n > 0) {
-          const int key = j.r0 + row;
+          const int key = j.r0() + row;
           zero = key >= cross_len(a.kv_lens, yb, a.kv_len) || (mask && !mask[key]);
         }
         for (int k = (i0 ^ c) & 1; k < n; k += 2) {
@@ -965,16 +973,16 @@ __global__ void __launch_bounds__(Grad<D, KV>::THREADS, 1)
     bool ok = true;
     // This thread's row of a job: offsets in X1 and X2, and in the gradients; false: there is no such row.
     const auto row_at = [&](const Job<KV>& j, long long& o1, long long& o2) {
-      const int r = j.r0 + row;
+      const int r = j.r0() + row;
       if (KV) {
         o1 = j.b * a.ks.b + j.hk * a.ks.h + r * a.ks.t;
         o2 = j.b * a.vs.b + j.hk * a.vs.h + r * a.vs.t;
         return r < a.kv_len;
       }
-      const int h = j.hk * j.group + r / a.q_len, t = r % a.q_len;
+      const int h = j.hk * p.group + r / a.q_len, t = r % a.q_len;
       o1 = j.b * a.qs.b + h * a.qs.h + t * a.qs.t;
       o2 = j.b * a.os.b + h * a.os.h + t * a.os.t;
-      return r < j.group * a.q_len && t < cross_len(a.q_lens, j.b, a.q_len);
+      return r < p.group * a.q_len && t < cross_len(a.q_lens, j.b, a.q_len);
     };
     // Rows go through shared memory, so that eight lanes move 128 bytes of one: a lane to a row in global
     // memory costs 32 transactions an access, and the warps that form P and dS wait behind them.
@@ -1044,45 +1052,43 @@ __global__ void __launch_bounds__(Grad<D, KV>::THREADS, 1)
         __syncwarp();
       }
     };
-    const auto next_job_quiet = [&](int job) {  // the next job with items, from `job` on
-      while (job < p.jobs && Job<KV>(p, job).count(a) == 0) job += grid;
-      return job;
+    const auto next_job_quiet = [&](Job<KV>& j) {  // to the next job with items
+      while (j.job < p.jobs && j.count(p) == 0) j.step(p);
     };
-    const auto next_job = [&](int job) {  // the next one with items, from `job` on; zeros for those without
-      for (; job < p.jobs; job += grid) {
-        const Job<KV> j(p, job);
-        if (j.count(a) > 0) break;
-        store_zeros(j);
-      }
-      return job;
+    const auto next_job = [&](Job<KV>& j) {  // ... with zeros for those without
+      for (; j.job < p.jobs && j.count(p) == 0; j.step(p)) store_zeros(j);
     };
     // The rows of the first NX jobs, then each time a job is done those of the one that takes its columns,
     // fetched while it runs.
-    int x = 0, job = next_job(blockIdx.x);
-    int ahead = job;  // the next job to fetch
-    const auto advance = [&] { ahead = next_job(ahead + grid); };
-    for (int k = 0; k < NX && ahead < p.jobs; ++k) {
-      fetch_rows(Job<KV>(p, ahead));
+    int x = 0;
+    Job<KV> j(p);
+    next_job(j);
+    Job<KV> ahead = j;  // the next job to fetch
+    const auto advance = [&] {
+      ahead.step(p);
+      next_job(ahead);
+    };
+    for (int k = 0; k < NX && ahead.job < p.jobs; ++k) {
+      fetch_rows(ahead);
       place_rows(k);
       advance();
     }
-    while (job < p.jobs) {
-      if (!L::X_SMEM && ahead < p.jobs) fetch_rows(Job<KV>(p, ahead));
-      const Job<KV> j(p, job);
+    while (j.job < p.jobs) {
+      if (!L::X_SMEM && ahead.job < p.jobs) fetch_rows(ahead);
       long long o[2];
       const bool in = !KV && row_at(j, o[0], o[1]);
       bool seen = true;
       if (KV && (a.kv_lens || a.key_mask)) {  // a masked key's gradient is 0 whatever its row holds
         seen = false;
-        for (int b = j.b; b < j.b_hi; ++b)
-          seen |= j.r0 + row < cross_len(a.kv_lens, b, a.kv_len) &&
-                  (!a.key_mask || a.key_mask[static_cast<long long>(b) * a.kv_len + min(j.r0 + row, a.kv_len - 1)]);
+        for (int b = j.b; b < j.b_hi(p); ++b)
+          seen |= j.r0() + row < cross_len(a.kv_lens, b, a.kv_len) &&
+                  (!a.key_mask || a.key_mask[static_cast<long long>(b) * a.kv_len + min(j.r0() + row, a.kv_len - 1)]);
       }
       // (These warps wait long: they sleep between polls and leave the issue slots to the others.)
       ok = mbar_wait_bounded_backoff(&st->done[x % NA], (x / NA) & 1, abort_flag, p.err, kErrCrossSoftmaxWait, 40);
       if (!__all_sync(0xffffffffu, ok)) break;
       tc_fence_after();
-      if (NX == 1 && ahead < p.jobs) place_rows(x + 1);
+      if (NX == 1 && ahead.job < p.jobs) place_rows(x + 1);
       // Sums: through the boxes, as many as there are at a time.
       constexpr int SUMS = (KV ? 2 : 1) * L::NCH;  // chunks of 64 columns: dv, then dk; or dq
 #pragma unroll
@@ -1117,10 +1123,10 @@ __global__ void __launch_bounds__(Grad<D, KV>::THREADS, 1)
           // 32 rows a box; the tensor maps end at kv_len and head_dim.
           fence_proxy_async_smem();
           __syncwarp();
-          if (lane == 0 && j.r0 + quarter * 32 < a.kv_len) {  // (no store starts past the tensor)
+          if (lane == 0 && j.r0() + quarter * 32 < a.kv_len) {  // (no store starts past the tensor)
             for (int h = h0; h < h0 + L::OUTS; ++h) {
               const bool v = h < L::NCH;
-              tma_store_4d(v ? &map_dv : &map_dk, out_box + (h - h0) * CH, h % L::NCH * 64, j.r0 + quarter * 32,
+              tma_store_4d(v ? &map_dv : &map_dk, out_box + (h - h0) * CH, h % L::NCH * 64, j.r0() + quarter * 32,
                            (v ? p.x2_head : p.x1_head) ? j.hk : 0, (v ? p.x2_batch : p.x1_batch) ? j.b : 0);
             }
             bulk_commit_group();
@@ -1141,9 +1147,10 @@ __global__ void __launch_bounds__(Grad<D, KV>::THREADS, 1)
           __syncwarp();
         }
       }
-      if (NX > 1 && ahead < p.jobs) place_rows(x + NX);
-      if (ahead < p.jobs) advance();
-      job = next_job_quiet(job + grid);
+      if (NX > 1 && ahead.job < p.jobs) place_rows(x + NX);
+      if (ahead.job < p.jobs) advance();
+      j.step(p);
+      next_job_quiet(j);
       ++x;
     }
     if (KV && lane == 0) bulk_wait_group0();  // shared memory outlives the stores' reads
@@ -1232,10 +1239,11 @@ cudaError_t bwd_tc(const CrossGradArgs& g, const float* neg_lse2, const float* n
     if (e != cudaSuccess) return e;
     const long long jobs = static_cast<long long>(tiles) * entries * a.hk;
     if (jobs > 0x7fffffffLL - ctx->sm_count) return cudaErrorNotSupported;
+    const int blocks = static_cast<int>(std::min<long long>(jobs, ctx->sm_count));
     const GradParams p{g,           neg_lse2,   neg_d,       q_pad,      y1.by_head,  y1.by_batch,
                        y2.by_head,  y2.by_batch, x1.by_head, x1.by_batch, x2.by_head, x2.by_batch,
-                       static_cast<int>(jobs), tiles, !KV && g.dk, a.scale * kLog2e, ctx->err_word};
-    const unsigned blocks = static_cast<unsigned>(std::min<long long>(jobs, ctx->sm_count));
+                       static_cast<int>(jobs), tiles, a.hq / a.hk, blocks % tiles, blocks / tiles % a.hk, blocks / tiles / a.hk,
+                       !KV && g.dk, a.scale * kLog2e, ctx->err_word};
     return launch_pdl(cross_grad_tc_kernel<D, KV>, dim3(blocks), dim3(L::THREADS), L::SMEM, s, y1.map, y2.map, x1.map, x2.map,
                       dk.map, dv.map, p);
   };
