@@ -9,7 +9,7 @@ namespace lcb {
 
 // Length of a batch entry, clamped to what the tensors hold.
 __device__ __forceinline__ int cross_len(const int* lens, int b, int most) {
-  return lens ? min(max(lens[b], 0), most) : most;
+  return lens ? min(max(__ldg(lens + b), 0), most) : most;
 }
 
 // Parts of a forward pass that is split along the keys: part i of row r (rows are dense

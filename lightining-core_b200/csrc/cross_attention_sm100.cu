@@ -545,7 +545,7 @@ __global__ void __launch_bounds__(Fwd<D>::THREADS, 1)
 //   * three issuing warps, for S, dP and the sums, which order each other by barriers only
 //   * resident blocks that go from job to job: four more warps load the next job's rows and store
 //     the last one's sums meanwhile (two sets of TMEM columns where they fit)
-// B200, row terms included: [16, 16, 512 x 2048 ragged, 64] 267 us (blocks of one job with one chain of products:
+// B200, row terms included: [16, 16, 512 x 2048 ragged, 64] 261 us (blocks of one job with one chain of products:
 // 471), [4, 16/4, 1024 x 2048 ragged, 128] 185 us (266).
 constexpr int QT = 64;         // rows of an item
 constexpr int QCH = QT * 128;  // one [64 rows x 64 bf16] box
@@ -600,7 +600,7 @@ struct GradParams {
 // A job's rows.  Its items are, in order: the batch entries [b, b_hi) with span() > 0, `heads` heads each, tiles
 // of 64 rows up to span().
 // A block goes from job to job by adding the grid's size in (batch entry, key head, tile) digits (with divisions
-// 270 and 188 us where it is 267 and 185).
+// 270 and 188 us below, without 267 and 185).
 template <bool KV>
 struct Job {
   int job, b, hk, tile;
