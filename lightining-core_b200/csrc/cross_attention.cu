@@ -12,6 +12,9 @@
 // K rows (stride DP + 4 words) fall on different banks, every global read is contiguous, and the
 // two inner products read 8 float4 for 64 FMAs.  Masked keys and rows past the end are staged as
 // zeros and their scores replaced, so what memory holds there never enters a sum.
+// Bound by shared-memory reads and issue slots.  B200, fp32: [4, 16, 333 x 1000, 64] 370 us (15 TFLOP/s), backward 782;
+// [4, 16, 333 x 1000, 200] 1486 us, backward 4500 (with tiles of 32 rows, 64 threads, 3560 and 16253: hence one buffer
+// for two operands above 128 columns, which leaves room for tiles of 64).
 // Rows of the heads that share a key head form one list (row = head-in-group * q_len + token), so
 // a tile of few queries is filled by its group.
 #include <cuda_bf16.h>
@@ -395,9 +398,10 @@ template <typename T, int DP, int TT>
 __global__ void __launch_bounds__(Tile<DP, TT>::NT) cross_dq_simt_kernel(CrossGradArgs g, const float* neg_lse2,
                                                                          const float* neg_d, int q_pad, int vec) {
   using L = Tile<DP, TT>;
+  constexpr bool ONE = DP > 128;  // one buffer for K and V
   const CrossArgs& a = g.f;
   extern __shared__ __align__(16) float smem[];
-  float *Q = smem, *G = Q + L::ROWS, *K = G + L::ROWS, *V = K + L::ROWS, *P = V + L::ROWS;
+  float *Q = smem, *G = Q + L::ROWS, *K = G + L::ROWS, *V = ONE ? K : K + L::ROWS, *P = V + L::ROWS;
   __shared__ unsigned char seen[TT];
   const int tid = threadIdx.x, rg = tid / L::GL, cg = tid % L::GL;
   const int group = a.hq / a.hk, rows = group * a.q_len;
@@ -440,12 +444,18 @@ __global__ void __launch_bounds__(Tile<DP, TT>::NT) cross_dq_simt_kernel(CrossGr
     __syncthreads();
     const auto visible = [&](int j) { return k0 + j < kv_end && (!mask || mask[k0 + j]); };
     if (tid < TT) seen[tid] = visible(tid);
-    stage<T, DP, TT>(K, kp, a.d, vec, [&](int j) -> long long { return visible(j) ? (k0 + j) * a.ks.t : -1; });
+    const auto k_off = [&](int j) -> long long { return visible(j) ? (k0 + j) * a.ks.t : -1; };
+    if (!ONE) stage<T, DP, TT>(K, kp, a.d, vec, k_off);
     stage<T, DP, TT>(V, vp, a.d, vec, [&](int j) -> long long { return visible(j) ? (k0 + j) * a.vs.t : -1; });
     __syncthreads();
     float s[4][4], dp[4][4];
-    dot_tile<DP, TT>(Q, K, rg, cg, s);
     dot_tile<DP, TT>(G, V, rg, cg, dp);
+    if (ONE) {
+      __syncthreads();
+      stage<T, DP, TT>(K, kp, a.d, vec, k_off);
+      __syncthreads();
+    }
+    dot_tile<DP, TT>(Q, K, rg, cg, s);
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
@@ -465,9 +475,11 @@ template <typename T, int DP, int TT, bool DK, bool DV>
 __global__ void __launch_bounds__(Tile<DP, TT>::NT) cross_dkv_simt_kernel(CrossGradArgs g, const float* neg_lse2,
                                                                           const float* neg_d, int q_pad, int vec) {
   using L = Tile<DP, TT>;
+  constexpr bool ONE = DP > 128;  // one buffer for Q and dout
+  static_assert(!ONE || DK != DV);
   const CrossArgs& a = g.f;
   extern __shared__ __align__(16) float smem[];
-  float *Q = smem, *G = Q + L::ROWS, *K = G + L::ROWS, *V = K + L::ROWS, *P = V + L::ROWS;
+  float *Q = smem, *G = ONE ? Q : Q + L::ROWS, *K = G + L::ROWS, *V = K + L::ROWS, *P = V + L::ROWS;
   __shared__ float row_lse[TT], row_del[TT];
   __shared__ unsigned char seen[TT];
   const int tid = threadIdx.x, rg = tid / L::GL, cg = tid % L::GL;
@@ -503,15 +515,20 @@ __global__ void __launch_bounds__(Tile<DP, TT>::NT) cross_dkv_simt_kernel(CrossG
         t = r % a.q_len;
         return r < rows && t < q_end;
       };
+      const auto stage_q = [&] {
+        stage<T, DP, TT>(Q, static_cast<const T*>(a.q), a.d, vec, [&](int r) -> long long {
+          int h, t;
+          return at(r, h, t) ? b * a.qs.b + h * a.qs.h + t * a.qs.t : -1;
+        });
+      };
+      const auto stage_g = [&] {
+        stage<T, DP, TT>(G, static_cast<const T*>(g.dout), a.d, vec, [&](int r) -> long long {
+          int h, t;
+          return at(r, h, t) ? b * a.os.b + h * a.os.h + t * a.os.t : -1;
+        });
+      };
+      float s[4][4], dp[4][4];
       __syncthreads();
-      stage<T, DP, TT>(Q, static_cast<const T*>(a.q), a.d, vec, [&](int r) -> long long {
-        int h, t;
-        return at(r, h, t) ? b * a.qs.b + h * a.qs.h + t * a.qs.t : -1;
-      });
-      stage<T, DP, TT>(G, static_cast<const T*>(g.dout), a.d, vec, [&](int r) -> long long {
-        int h, t;
-        return at(r, h, t) ? b * a.os.b + h * a.os.h + t * a.os.t : -1;
-      });
       if (tid < TT) {
         int h, t;
         const bool in = at(tid, h, t);
@@ -519,8 +536,15 @@ __global__ void __launch_bounds__(Tile<DP, TT>::NT) cross_dkv_simt_kernel(CrossG
         row_lse[tid] = in ? neg_lse2[w] : -INFINITY;
         row_del[tid] = in ? neg_d[w] : 0.0f;
       }
+      if (!ONE || DK) stage_g();
+      if (!ONE) stage_q();
+      if (ONE && DK) {  // dout gives way to Q
+        __syncthreads();
+        dot_tile<DP, TT>(V, G, rg, cg, dp);
+        __syncthreads();
+      }
+      if (ONE) stage_q();
       __syncthreads();
-      float s[4][4], dp[4][4];
       dot_tile<DP, TT>(K, Q, rg, cg, s);  // rows are keys here
 #pragma unroll
       for (int i = 0; i < 4; ++i)
@@ -532,12 +556,18 @@ __global__ void __launch_bounds__(Tile<DP, TT>::NT) cross_dkv_simt_kernel(CrossG
         for (int i = 0; i < 4; ++i)
 #pragma unroll
           for (int j = 0; j < 4; ++j) P[(rg + i * L::GL) * L::LP + cg + j * L::GL] = s[i][j];
+        if (ONE) {  // Q gives way to dout
+          __syncthreads();
+          stage_g();
+        }
         __syncthreads();
         acc_tile<DP, TT>(P, G, rg, cg, dv);
       }
       if constexpr (DK) {
-        dot_tile<DP, TT>(V, G, rg, cg, dp);
-        __syncthreads();  // the weights are used up
+        if (!ONE) {
+          dot_tile<DP, TT>(V, G, rg, cg, dp);
+          __syncthreads();  // the weights are used up
+        }
 #pragma unroll
         for (int i = 0; i < 4; ++i)
 #pragma unroll
@@ -580,7 +610,7 @@ cudaError_t fwd_simt(const CrossArgs& a, cudaStream_t s) {
   const long long blocks = (rows + TT - 1) / TT * a.batch * a.hk;
   if (blocks > 0x7fffffffLL) return cudaErrorNotSupported;
   CrossSplitWork w;
-  e = w.begin(a, blocks, TT, 2, s);
+  e = w.begin(a, blocks, TT, 1, 2, s);
   if (e != cudaSuccess) return e;
   const int vec = vec4(a.q, a.qs, a.d, sizeof(T)) && vec4(a.k, a.ks, a.d, sizeof(T)) && vec4(a.v, a.vs, a.d, sizeof(T));
   cross_fwd_simt_kernel<T, DP, TT>
@@ -592,14 +622,15 @@ template <typename T>
 cudaError_t fwd_simt_any(const CrossArgs& a, cudaStream_t s) {
   if (a.d <= 64) return fwd_simt<T, 64, 64>(a, s);
   if (a.d <= 128) return fwd_simt<T, 128, 64>(a, s);
-  return fwd_simt<T, 256, 32>(a, s);
+  return fwd_simt<T, 256, 64>(a, s);
 }
 
 template <typename T, int DP, int TT>
 cudaError_t bwd_simt(const CrossGradArgs& g, const float* neg_lse2, const float* neg_d, int q_pad, cudaStream_t s) {
   using L = Tile<DP, TT>;
   const CrossArgs& a = g.f;
-  constexpr size_t SMEM = (4 * L::ROWS + L::SQ) * sizeof(float);
+  constexpr size_t SMEM = ((DP > 128 ? 3 : 4) * L::ROWS + L::SQ) * sizeof(float);
+  static_assert(SMEM <= 227 * 1024 - 1024);
   const int vec = vec4(a.q, a.qs, a.d, sizeof(T)) && vec4(a.k, a.ks, a.d, sizeof(T)) &&
                   vec4(a.v, a.vs, a.d, sizeof(T)) && vec4(g.dout, a.os, a.d, sizeof(T));
   cudaError_t e = cudaSuccess;
@@ -669,20 +700,23 @@ cudaError_t bwd_any(const CrossGradArgs& g, cudaStream_t s) {
   else if (e == cudaSuccess)
     e = a.d <= 64    ? bwd_simt<T, 64, 64>(g, neg_lse2, neg_d, q_pad, s)
         : a.d <= 128 ? bwd_simt<T, 128, 64>(g, neg_lse2, neg_d, q_pad, s)
-                     : bwd_simt<T, 256, 32>(g, neg_lse2, neg_d, q_pad, s);
+                     : bwd_simt<T, 256, 64>(g, neg_lse2, neg_d, q_pad, s);
   const cudaError_t f = workspace_free(ws, s);
   return e != cudaSuccess ? e : f;
 }
 
 }  // namespace
 
-// Splits a problem of `blocks` row tiles along its key tiles (of `tile` keys) when the blocks alone
-// leave SMs idle: as many parts as fill `per_sm` blocks to an SM, at least one key tile each.
-cudaError_t CrossSplitWork::begin(const CrossArgs& a, long long blocks, int tile, int per_sm, cudaStream_t s) {
+// Splits a problem of `blocks` row tiles along its key tiles (of `tile` keys) when the blocks alone leave SMs idle: as
+// many parts as fill `per_sm` blocks to an SM, at least `least` key tiles each -- a part's fill, drain and join must
+// not cost more than it saves.  B200, bf16 (128 keys a tile): [1, 8, 64 x 4000, 128] 25 us split, 60 not; [2, 8, 512 x
+// 512, 64] 23 in parts of one tile, 16.6 whole.  fp32 (64 keys): [1, 8, 100 x 1000, 64] 21 us, 25 in parts of one tile,
+// 33 whole; on the CUDA cores [1, 8, 100 x 1000, 200] 118 in parts of one tile, 746 whole.
+cudaError_t CrossSplitWork::begin(const CrossArgs& a, long long blocks, int tile, int least, int per_sm, cudaStream_t s) {
   DeviceCtx* ctx = device_ctx();
   if (!ctx) return cudaErrorNoDevice;
   const long long tiles = (a.kv_len + tile - 1) / tile, room = static_cast<long long>(per_sm) * ctx->sm_count;
-  return begin_parts(a, std::min<long long>({room / blocks, tiles, 64}), s);
+  return begin_parts(a, std::min<long long>({room / blocks, tiles / least, 64}), s);
 }
 
 cudaError_t CrossSplitWork::begin_parts(const CrossArgs& a, long long n, cudaStream_t s) {

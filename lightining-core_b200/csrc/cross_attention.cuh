@@ -25,7 +25,7 @@ struct CrossSplit {
 struct CrossSplitWork {
   CrossSplit sp{};
   void* ws = nullptr;
-  cudaError_t begin(const CrossArgs& a, long long blocks, int tile, int per_sm, cudaStream_t s);
+  cudaError_t begin(const CrossArgs& a, long long blocks, int tile, int least, int per_sm, cudaStream_t s);
   cudaError_t begin_parts(const CrossArgs& a, long long n, cudaStream_t s);  // n parts (at most 1: none)
   cudaError_t end(const CrossArgs& a, cudaError_t launched, cudaStream_t s);
 };

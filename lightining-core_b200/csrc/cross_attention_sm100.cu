@@ -1207,7 +1207,7 @@ cudaError_t fwd_tc(const CrossArgs& a, cudaStream_t s) {
   const long long blocks = (rows + 2 * TILE - 1) / (2 * TILE) * a.batch * a.hk;
   if (blocks > 0x7fffffffLL) return cudaErrorNotSupported;
   CrossSplitWork w;
-  if ((e = w.begin(a, blocks, TILE, 1, s)) != cudaSuccess) return e;
+  if ((e = w.begin(a, blocks, TILE, 3, 1, s)) != cudaSuccess) return e;
   const FwdParams p{a, w.sp, mk.by_head, mk.by_batch, mv.by_head, mv.by_batch, a.scale * kLog2e, ctx->err_word};
   cross_fwd_tc_kernel<D>
       <<<dim3(static_cast<unsigned>(blocks), w.sp.splits), F::THREADS, F::SMEM, s>>>(mk.map, mv.map, p);

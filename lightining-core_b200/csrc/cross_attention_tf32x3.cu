@@ -863,7 +863,7 @@ cudaError_t fwd_f32(const CrossArgs& a, cudaStream_t s) {
     e = cudaErrorInvalidValue;
   if (e == cudaSuccess) {
     CrossSplitWork w;
-    e = w.begin(a, blocks, F::T, 1, s);
+    e = w.begin(a, blocks, F::T, 2, 1, s);
     if (e == cudaSuccess) {
       const int vec = rows4(a.q, a.qs, a.d) && rows4(a.k, a.ks, a.d) && rows4(a.v, a.vs, a.d);
       cross_split_kernel<D><<<dim3(z.q_blocks + 2 * z.k_blocks, z.pairs), 256, 0, s>>>(a, job, vec);
