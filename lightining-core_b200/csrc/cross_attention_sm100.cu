@@ -798,8 +798,12 @@ __global__ void __launch_bounds__(Grad<D, KV>::THREADS, 1)
             if (!(ok = wait(&st->full[s], (i / NS) & 1))) break;
             // Rows that memory holds but that do not count are zeroed: their weights are 0, but a NaN
             // would enter the sums all the same (Y2 of the dq walk, V, enters none).
-            if ((KV || !which) && (mask || (t0 + QT > y_end && y_end < y_len)))
-              scrub_rows<L::NCH, QT>(y, [&](int r) { return t0 + r < y_end && (!mask || mask[t0 + r]); });
+            if ((KV || !which) && (mask || (t0 + QT > y_end && y_end < y_len))) {
+              const auto keep = [&](int r) { return t0 + r < y_end && (!mask || mask[t0 + r]); };
+              scrub_rows<L::NCH, QT>(y, keep);
+              // dv reads Y2 as soon as P is there, which waits for S and not for dP: here too, whoever comes first.
+              if (KV && !which) scrub_rows<L::NCH, QT>(sY2(s), keep);
+            }
             if (i > 0 && !(ok = wait(read, (i - 1) & 1))) break;
             tc_fence_after();
             const uint64_t bd = smem_desc_sw128(smem_u32(y), 16, 1024);
