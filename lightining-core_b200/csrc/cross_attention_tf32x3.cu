@@ -511,7 +511,7 @@ struct Grad {
   static constexpr int R_OFF = D / 32 * ACH * 2, TAIL_OFF = R_OFF + NP * PIECE;
   struct Tail {
     float2 terms[2][T];
-    uint64_t a_full, x_full, full[NP], used[NP], s_full, dp_full, p_full, ds_full, o_full, o_free, drain;
+    uint64_t a_full, x_full, full[NP], used[NP], t_full[2], s_full, dp_full, p_full, ds_full, o_full, o_free, drain;
     uint32_t tmem_base;
     int abort_flag;
   };
@@ -574,6 +574,7 @@ __global__ void __launch_bounds__(GRAD_THREADS, 1) cross_grad_f32_tc_kernel(cons
       mbar_init(&st->full[i], 1);
       mbar_init(&st->used[i], 1);
     }
+    for (int i = 0; i < 2; ++i) mbar_init(&st->t_full[i], 1);
     mbar_init(&st->s_full, 1);
     mbar_init(&st->dp_full, 1);
     mbar_init(&st->p_full, 8);
@@ -612,14 +613,18 @@ __global__ void __launch_bounds__(GRAD_THREADS, 1) cross_grad_f32_tc_kernel(cons
         return true;
       };
       bool ok = true;
+      int terms = 0;
       for (int j = 0; j < n && ok; ++j) {
         const int t0 = j * T;
-        if (!(ok = room(keys ? PIECE + T * sizeof(float2) : PIECE))) break;
+        if (!(ok = room(PIECE))) break;
         load_piece<D, false>(slot(i), keys ? &p.qr : &p.kr, t0, pair, p.pairs, &st->full[i % NP]);
         // (A buffer of terms is written two tiles later, when pieces behind its tile's last product were read.)
-        if (keys)
+        if (keys) {
+          mbar_arrive_expect_tx(&st->t_full[j & 1], T * sizeof(float2));
           bulk_load(st->terms[j & 1], p.terms + static_cast<long long>(pair) * p.rows_pad + t0, T * sizeof(float2),
-                    &st->full[i % NP]);
+                    &st->t_full[j & 1]);
+          ++terms;
+        }
         ++i;
         if (with_ds) {
           if (!(ok = room(PIECE))) break;
@@ -640,6 +645,7 @@ __global__ void __launch_bounds__(GRAD_THREADS, 1) cross_grad_f32_tc_kernel(cons
       if (!ok) {
         drain_bar(&st->a_full, 0);
         for (int k = max(0, i - NP); k < i; ++k) drain_bar(&st->full[k % NP], (k / NP) & 1);
+        for (int k = max(0, terms - 2); k < terms; ++k) drain_bar(&st->t_full[k & 1], (k >> 1) & 1);
       }
     }
   } else if (warp == 1) {
@@ -732,6 +738,7 @@ __global__ void __launch_bounds__(GRAD_THREADS, 1) cross_grad_f32_tc_kernel(cons
         const int k = j * T + half * SC + lane;
         if (mask || (j + 1) * T > kv_end) vis = __ballot_sync(0xffffffffu, lane < SC && k < kv_end && (!mask || mask[k]));
       }
+      if (keys && !(ok = wait(&st->t_full[ph], (j >> 1) & 1))) break;
       if (!(ok = wait(&st->s_full, ph))) break;
       tc_fence_after();
       uint32_t w[SC];
