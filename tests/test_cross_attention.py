@@ -173,10 +173,17 @@ class Case:
                                             self.lc.BF16 if self.r != U else self.lc.F32, self.qs, self.ks, self.vs,
                                             self.os, p(self.q_lens), p(self.kv_lens), p(self.key_mask), self.scale)
 
+    def after_fills(self, stream):
+        """A stream of the caller's waits for what was written on torch's."""
+        cur = self.torch.cuda.current_stream()
+        if stream is not None and stream != cur.cuda_stream:
+            self.torch.cuda.ExternalStream(stream).wait_stream(cur)
+
     def forward(self, stream=None, want_lse=True):
         torch = self.torch
         self.out_mem, self.out = self.like(self.dout)
         self.lse = torch.full((self.b, self.hq, self.nq), HOLE, device="cuda")
+        self.after_fills(stream)
         self.lc.check(self.lc.lib.lcCrossAttentionForward(self.desc(), self.q.data_ptr(), self.k.data_ptr(),
                                                           self.v.data_ptr(), self.out.data_ptr(),
                                                           self.lse.data_ptr() if want_lse else None, None, stream))
@@ -185,6 +192,7 @@ class Case:
     def backward(self, out, lse, dq=True, dkv=True, stream=None):
         self.mem, grads = zip(*(self.like(x) for x in (self.q, self.k, self.v)))
         p = [g.data_ptr() for g in grads]
+        self.after_fills(stream)
         self.lc.check(self.lc.lib.lcCrossAttentionBackward(
             self.desc(), self.dout.data_ptr(), self.q.data_ptr(), self.k.data_ptr(), self.v.data_ptr(), out.data_ptr(),
             lse.data_ptr(), p[0] if dq else None, p[1] if dkv else None, p[2] if dkv else None, stream))
