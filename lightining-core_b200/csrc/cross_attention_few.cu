@@ -13,8 +13,9 @@
 // fp32, at most 8 rows, head_dim <= 128 (tiles of 4096 / D keys): the CUDA cores, 2 * D * rows FMAs a key against 8 * D
 // bytes, are faster than the bytes.  A quad takes a key's dot products (the rows of Q in shared memory), then every
 // lane four columns of O.
-// A block's warps join their (maximum, sum, O) in shared memory; the keys of a pair are split over a cluster of up to 8 blocks, which join theirs through distributed shared memory -- one
-// launch, no workspace -- and over several clusters (and cross_combine) only when pairs are very few.
+// A block's warps join their (maximum, sum, O) in shared memory; the keys of a pair are split over a cluster of up to
+// 8 blocks, which join theirs through distributed shared memory -- one launch, no workspace -- and over several
+// clusters (and the join of parts) only when pairs are very few.
 // B200, 64 sequences of 32 / 8 heads over 2048..4096 keys, head_dim 128 (811 MB, floor 126 us): loads straight
 // into registers, three blocks to an SM, 226 us; the tiled tensor-core kernel 202 us (two stages of 64 KB do not cover
 // the latency); this one 142 us (with 4 blocks to a pair instead of 2: 154, with 8: 195).
@@ -239,7 +240,8 @@ __global__ void __launch_bounds__(THREADS, 2)
       const __nv_bfloat16* src = static_cast<const __nv_bfloat16*>(a.q) + job.b * a.qs.b +
                                  (job.hk * job.group + row / a.q_len) * a.qs.h + row % a.q_len * a.qs.t + c * 8;
 #pragma unroll
-      for (int n = 0; n < NB; ++n) q[n][r] = job.live(a, row) ? __ldg(reinterpret_cast<const uint4*>(src + n * 32)) : make_uint4(0, 0, 0, 0);
+      for (int n = 0; n < NB; ++n)
+        q[n][r] = job.live(a, row) ? __ldg(reinterpret_cast<const uint4*>(src + n * 32)) : make_uint4(0, 0, 0, 0);
     }
     const float sc = a.scale * kLog2e;
     // Piece k of 16 bytes of this warp's key r in a box.

@@ -63,14 +63,14 @@ __device__ __forceinline__ void scrub_rows(uint8_t* tile, Keep keep) {
   __syncwarp();
 }
 
-// Whether this lane's keys of the tile at kv0 (kv0 + step i + lane) are visible; a ballot of byte[i]
+// Whether this lane's keys of the tile at kv0 (kv0 + 64 i + lane) are visible; a ballot of byte[i]
 // gives every lane the word of those 32 keys.  Loaded ahead of the wait for the scores.
 template <int N>
 __device__ __forceinline__ void load_mask_bytes(const unsigned char* mask, int kv0, int kv_end, int lane,
-                                                unsigned char (&byte)[N], int step = 32) {
+                                                unsigned char (&byte)[N]) {
 #pragma unroll
   for (int i = 0; i < N; ++i) {
-    const int k = kv0 + i * step + lane;
+    const int k = kv0 + i * 64 + lane;
     byte[i] = k < kv_end && (!mask || mask[k]);
   }
 }
@@ -292,8 +292,8 @@ __global__ void __launch_bounds__(Fwd<D>::THREADS, 1)
       };
       const auto next_keys = [&] { return j + 1 >= n || wait(&st->k_full[(j + 1) % NS], ((j + 1) / NS) & 1); };
       if constexpr (F::OWN_P) {
-        // Tile B is half a step behind A (its first scores wait for A's first weights): one tile's exponentials run beside the rest of the
-        // other's softmax.
+        // Tile B is half a step behind A (its first scores wait for A's first weights): one tile's exponentials
+        // run beside the rest of the other's softmax.
         if (warp == 1) {
           if (j + 1 == n || !(ok = next_keys())) break;
           for (int h = 0; h < 2 && ok; ++h)  // s_read[h] next completes for S_h(j+1)
@@ -380,7 +380,7 @@ __global__ void __launch_bounds__(Fwd<D>::THREADS, 1)
       for (int j = 0; j < n; ++j) {
         const int kv0 = (t_lo + j) * TILE;
         const bool partial = mask || kv0 + TILE > kv_end;
-        if (partial) load_mask_bytes(mask, kv0 + half * 32, kv_end, lane, byte, 64);
+        if (partial) load_mask_bytes(mask, kv0 + half * 32, kv_end, lane, byte);
         // s_full[h] next completes for S_h(j+1), which needs P_h(j) from these warps first.
         if (!(ok = warp_wait_ready(&st->s_full[h], j & 1, abort_flag, p.err, kErrCrossSoftmaxWait))) break;
         tc_fence_after();
@@ -1187,7 +1187,8 @@ bool head_map(HeadMap* m, const void* base, const HeadStrides& s, int batch, int
   const cuuint64_t strides[3] = {row, m->by_head ? static_cast<cuuint64_t>(s.h) * es : row,
                                  m->by_batch ? static_cast<cuuint64_t>(s.b) * es : row};
   const cuuint32_t box[4] = {static_cast<cuuint32_t>(128 / es), static_cast<cuuint32_t>(box_rows), 1, 1}, estr[4] = {1, 1, 1, 1};
-  return enc(&m->map, es == 2 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, const_cast<void*>(base), dims, strides, box, estr,
+  return enc(&m->map, es == 2 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4,
+             const_cast<void*>(base), dims, strides, box, estr,
              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
