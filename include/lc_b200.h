@@ -358,6 +358,7 @@ typedef struct lcCrossAttentionDesc {
  * queries and keys of different lengths, shared key heads, strides and masks.  A row without a visible
  * key is 0.  lse (fp32, dense [batch, q_heads, q_len], may be NULL) receives the log of each row's
  * sum of exp(scale * q k^T) (-infinity for a row without a visible key), which the backward pass needs.
+ * A row with a visible score of NaN or +infinity, or with -infinity for all of them, is NaN, and its lse too.
  * f32: fp32 arithmetic (on the tensor cores each product is the sum of three of its operands' high and low
  * halves, off by 2^-22 of its magnitude at most; visible infinities come out as NaN there); bf16: fp32
  * accumulation and softmax statistics, weights rounded to bf16; head_dim <= 256.  k and v may be broadcast over the batch (batch stride 0 with the other strides set: one source

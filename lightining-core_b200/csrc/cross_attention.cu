@@ -30,7 +30,6 @@ namespace lcb {
 namespace {
 
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kLn2 = 0.6931471805599453f;
 
 template <typename T>
 __device__ __forceinline__ float to_f(T v) { return static_cast<float>(v); }
@@ -198,7 +197,7 @@ __global__ void __launch_bounds__(Tile<DP, TT>::NT) cross_fwd_simt_kernel(CrossA
 #pragma unroll
     for (int c = 0; c < L::CPT; ++c) o[i][c] = 0.0f;
   }
-  const float sc = a.scale * kLog2e;
+  const float sc = a.scale * kLog2e, floor = cross_floor(sc);
   const T* kp = static_cast<const T*>(a.k) + b * a.ks.b + hk * a.ks.h;
   const T* vp = static_cast<const T*>(a.v) + b * a.vs.b + hk * a.vs.h;
   const unsigned char* mask = a.key_mask ? a.key_mask + static_cast<long long>(b) * a.kv_len : nullptr;
@@ -220,8 +219,10 @@ __global__ void __launch_bounds__(Tile<DP, TT>::NT) cross_fwd_simt_kernel(CrossA
       float mx = -INFINITY;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        if (!seen[cg + j * L::GL]) s[i][j] = -INFINITY;
-        mx = fmaxf(mx, s[i][j]);
+        if (seen[cg + j * L::GL])
+          mx = fmaxf(mx, fmaxf(s[i][j], floor));
+        else
+          s[i][j] = -INFINITY;
       }
       mx = fmaxf(m[i], lanes_max<L::GL>(mx) * sc);
       const float base = mx == -INFINITY ? 0.0f : mx;  // nothing visible yet: every weight is 0
@@ -262,11 +263,10 @@ __global__ void __launch_bounds__(Tile<DP, TT>::NT) cross_fwd_simt_kernel(CrossA
   }
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    f[i] = m[i] == -INFINITY ? 0.0f : 1.0f / l[i];
+    f[i] = cross_inverse(m[i], l[i]);
     int h, tt;
     const int r = rg + i * L::GL;
-    if (cg == 0 && a.lse && at(r, h, tt))
-      a.lse[row_of + r] = m[i] == -INFINITY ? -INFINITY : (m[i] + log2f(l[i])) * kLn2;
+    if (cg == 0 && a.lse && at(r, h, tt)) a.lse[row_of + r] = cross_lse(m[i], l[i]);
   }
   store_rows<T, DP, TT>(static_cast<T*>(a.out), o, f, a.d, rg, cg, [&](int r) -> long long {
     int h, t;
@@ -295,14 +295,14 @@ __global__ void __launch_bounds__(256) cross_combine_kernel(CrossArgs a, CrossSp
     l = fmaf(ml.y, exp2f(ml.x - base), l);
   }
   l = lanes_sum<32>(l);
-  const float inv = m == -INFINITY ? 0.0f : 1.0f / l;
+  const float inv = cross_inverse(m, l);
   T* out = static_cast<T*>(a.out) + b * a.os.b + h * a.os.h + t * a.os.t;
   float acc[8];  // head_dim <= 256
 #pragma unroll
   for (int c = 0; c < 8; ++c) acc[c] = 0.0f;
   for (int i = 0; i < sp.splits; ++i) {
-    const float w = exp2f(sp.ml[i * sp.rows + row].x - base);
-    if (w == 0.0f) continue;  // a part without a visible key
+    const float mi = sp.ml[i * sp.rows + row].x, w = exp2f(mi - base);
+    if (mi == -INFINITY) continue;  // a part without a visible key
     const float* o = sp.o + (static_cast<long long>(i) * sp.rows + row) * a.d;
 #pragma unroll
     for (int c = 0; c < 8; ++c)
@@ -311,7 +311,7 @@ __global__ void __launch_bounds__(256) cross_combine_kernel(CrossArgs a, CrossSp
 #pragma unroll
   for (int c = 0; c < 8; ++c)
     if (c * 32 + lane < a.d) out[c * 32 + lane] = from_f<T>(acc[c] * inv);
-  if (lane == 0 && a.lse) a.lse[row] = m == -INFINITY ? -INFINITY : (m + log2f(l)) * kLn2;
+  if (lane == 0 && a.lse) a.lse[row] = cross_lse(m, l);
 }
 
 // ---- backward -------------------------------------------------------------------------------

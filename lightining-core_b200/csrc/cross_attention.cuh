@@ -2,6 +2,7 @@
 #pragma once
 
 #include <cuda.h>
+#include <math.h>
 
 #include "lc_internal.hpp"
 
@@ -12,9 +13,27 @@ __device__ __forceinline__ int cross_len(const int* lens, int b, int most) {
   return lens ? min(max(__ldg(lens + b), 0), most) : most;
 }
 
+// A row's maximum (log2 domain) is -infinity if it has seen no key, and kCrossLowest at least if it has.  The maximum
+// itself drops NaN, so a row whose scores are all NaN would look like one without a key; with this floor its sum,
+// which is NaN, reaches the result.  cross_floor: the same floor in scores, before the scale `sc`.
+constexpr float kCrossLowest = -3.4e38f;
+__device__ __forceinline__ float cross_floor(float sc) { return kCrossLowest / fmaxf(sc, 1.0f); }
+
+// A row's factor and log-sum-exp from its maximum and sum.  A sum of 0 below a maximum that is not -infinity means
+// visible scores that are all -infinity: no softmax, NaN.
+__device__ __forceinline__ float cross_inverse(float m, float l) {
+  if (m == -INFINITY) return 0.0f;
+  return l == 0.0f ? NAN : 1.0f / l;
+}
+__device__ __forceinline__ float cross_lse(float m, float l) {
+  if (m == -INFINITY) return -INFINITY;
+  return l == 0.0f ? NAN : (m + log2f(l)) * 0.6931471805599453f;
+}
+
 // Parts of a forward pass that is split along the keys: part i of row r (rows are dense
 // [batch, q_heads, q_len]) holds the unnormalised sum o[i][r][.] of exp2(s - m) v over its keys and
-// ml[i][r] = (m, sum of exp2(s - m)), m the part's maximum of the scores in the log2 domain.
+// ml[i][r] = (m, sum of exp2(s - m)), m the part's maximum of the scores in the log2 domain (-infinity: no visible
+// key; the sums are 0 then).
 struct CrossSplit {
   int splits;
   long long rows;

@@ -38,7 +38,6 @@ namespace lcb {
 namespace {
 
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kLn2 = 0.6931471805599453f;
 constexpr int WARPS = 4;
 constexpr int ROWS = 16, ROWS_F32 = 8;
 constexpr int THREADS = (WARPS + 1) * 32;
@@ -204,8 +203,8 @@ __device__ __forceinline__ void few_join(FewSmem<D, R>& sm, const CrossArgs& a, 
       if (col == 0) sp.ml[part_row] = make_float2(mx, sum);
       continue;
     }
-    put4(static_cast<T*>(a.out) + job.b * a.os.b + h * a.os.h + tok * a.os.t + col, t, mx == -INFINITY ? 0.0f : 1.0f / sum);
-    if (col == 0 && a.lse) a.lse[at] = mx == -INFINITY ? -INFINITY : (mx + log2f(sum)) * kLn2;
+    put4(static_cast<T*>(a.out) + job.b * a.os.b + h * a.os.h + tok * a.os.t + col, t, cross_inverse(mx, sum));
+    if (col == 0 && a.lse) a.lse[at] = cross_lse(mx, sum);
   }
   if (cluster > 1) cl.sync();  // no block leaves while another reads its sums
 }
@@ -229,6 +228,7 @@ __global__ void __launch_bounds__(THREADS, 2)
   if (threadIdx.x == 0) few_init<L>(bars, &map_k, &map_v);
   __syncthreads();
   float o[NW * 8][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
+  bool saw = false;  // a visible key
   if (warp == WARPS) {
     if (lane == 0) few_load<L, __nv_bfloat16>(ring, bars, &map_k, &map_v, job, ax, err);
   } else {
@@ -261,6 +261,7 @@ __global__ void __launch_bounds__(THREADS, 2)
 #pragma unroll
           for (int e = 0; e < 2; ++e) vis_v[t * 2 + e] = vis[t][e] = job.seen(k0 + t * 8 + 2 * c + e);
       }
+      saw |= vis[0][0] | vis[0][1] | vis[1][0] | vis[1][1];
       if (!warp_wait_poll(&bars.full[st], (i / NS) & 1, &bars.abort_flag, err, kErrCrossSoftmaxWait)) break;
       const uint8_t *kbox = ring + st * STAGE, *vbox = kbox + NW * BOX;
       float s[2][4];
@@ -333,8 +334,10 @@ __global__ void __launch_bounds__(THREADS, 2)
   // The block's sums, over the ring (all its copies have landed and been read): every warp scales its own to the
   // common maximum.
   __syncthreads();
+  saw = __any_sync(0xffffffffu, saw);
 #pragma unroll
   for (int r = 0; r < 2; ++r) {
+    if (saw) m[r] = fmaxf(m[r], kCrossLowest);
     l[r] = quad_sum(l[r]);
     if (c == 0 && warp < WARPS) {
       sm.m[warp][g + 8 * r] = m[r];
@@ -396,6 +399,7 @@ __global__ void __launch_bounds__(THREADS, 2)
   __syncthreads();
   float4 o[R];
   float m[R], l[R];
+  bool saw = false;  // a visible key
 #pragma unroll
   for (int r = 0; r < R; ++r) {
     o[r] = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -418,6 +422,7 @@ __global__ void __launch_bounds__(THREADS, 2)
       for (int k = 0; k < KG; ++k) {
         mine[k] = !partial || job.seen(k0 + k * 8 + g);
         vis[k] = __ballot_sync(0xffffffffu, mine[k]);
+        saw |= vis[k] != 0;
       }
       if (!warp_wait_poll(&bars.full[st], (i / NS) & 1, &bars.abort_flag, err, kErrCrossSoftmaxWait)) break;
       const uint8_t *kbox = ring + st * STAGE, *vbox = kbox + NW * BOX;
@@ -497,6 +502,7 @@ __global__ void __launch_bounds__(THREADS, 2)
     }
 #pragma unroll
     for (int r = 0; r < R; ++r) {
+      if (saw) m[r] = fmaxf(m[r], kCrossLowest);
 #pragma unroll
       for (int d = 4; d < 32; d *= 2) l[r] += __shfl_xor_sync(0xffffffffu, l[r], d);
       if constexpr (CL == 16) {

@@ -20,7 +20,6 @@ void* tensor_map_encoder();
 namespace {
 
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kLn2 = 0.6931471805599453f;
 constexpr int TILE = 128;               // rows and keys of a tile
 constexpr int CH = 128 * 128;           // one [128 rows x 64 bf16] box, 128-byte swizzle: 16 KB
 
@@ -350,6 +349,7 @@ __global__ void __launch_bounds__(Fwd<D>::THREADS, 1)
       const uint32_t p_tmem = tmem + lane_base + F::P_COL + h * F::P_STEP + half * 16;
       const uint32_t o_tmem = tmem + lane_base + F::O_COL + h * F::O_STEP;
       constexpr int OC = D / 2;
+      const float floor = cross_floor(p.scale_log2);
       float m = -INFINITY, l = 0.0f;
       bool ok = true;
       unsigned char byte[2];
@@ -392,10 +392,13 @@ __global__ void __launch_bounds__(Fwd<D>::THREADS, 1)
           __syncwarp();
           if (lane == 0) mbar_arrive(&st->s_read[h]);
         }
+        float lowest = floor;  // of the maximum, unless this half sees no key
         if (partial) {
+          lowest = -INFINITY;
 #pragma unroll
           for (int c = 0; c < 2; ++c) {
             const unsigned w = __ballot_sync(0xffffffffu, byte[c]);
+            if (w) lowest = floor;
 #pragma unroll
             for (int e = 0; e < 32; ++e)
               if (!((w >> e) & 1u)) r[c][e] = __float_as_uint(-INFINITY);
@@ -407,7 +410,7 @@ __global__ void __launch_bounds__(Fwd<D>::THREADS, 1)
 #pragma unroll
         for (int e = 8; e < 64; e += 2)
           pm[(e >> 1) & 7] = max3(pm[(e >> 1) & 7], __uint_as_float(r[e >> 5][e & 31]), __uint_as_float(r[e >> 5][(e & 31) + 1]));
-        float mx = max3(max3(pm[0], pm[1], pm[2]), max3(pm[3], pm[4], pm[5]), fmaxf(pm[6], pm[7])), mo;
+        float mx = max3(max3(pm[0], pm[1], pm[2]), max3(pm[3], pm[4], pm[5]), max3(pm[6], pm[7], lowest)), mo;
         if (!(ok = swap(static_cast<uint32_t>(j), mx, &mo))) break;
         mx = fmaxf(mx, mo) * p.scale_log2;
         const bool need = mx > m + kRescale;
@@ -435,7 +438,7 @@ __global__ void __launch_bounds__(Fwd<D>::THREADS, 1)
           }
           tmem_wait_st();
         }
-        // A row that has seen no key yet has m = -inf: every score is -inf too and its weights are 0.
+        // A row that has seen no key yet has m = -inf: every score is -inf too and its weights are 0 (cross_floor).
         const float mu = m == -INFINITY ? 0.0f : m;
         const uint64_t sc2 = pk2(p.scale_log2, p.scale_log2), nm2 = pk2(-mu, -mu);
         uint64_t ps2[4] = {0, 0, 0, 0};
@@ -470,15 +473,15 @@ __global__ void __launch_bounds__(Fwd<D>::THREADS, 1)
         tc_fence_after();
         const int rr = base + row, g = rr / a.q_len, t = rr % a.q_len;
         const bool store = rr < rows && t < q_end;
-        const bool empty = m == -INFINITY;
+        const bool empty = m == -INFINITY;  // no visible key
         const long long at = (static_cast<long long>(b) * a.hq + hk * group) * a.q_len + rr;  // dense row
         const bool split = p.sp.splits > 1;
-        const float inv = split ? 1.0f : empty ? 0.0f : 1.0f / l;
+        const float inv = split ? 1.0f : cross_inverse(m, l);
         if (store && half == 0) {
           if (split)
             p.sp.ml[static_cast<long long>(blockIdx.y) * p.sp.rows + at] = make_float2(m, empty ? 0.0f : l);
           else if (a.lse)
-            a.lse[at] = empty ? -INFINITY : (m + log2f(l)) * kLn2;
+            a.lse[at] = cross_lse(m, l);
         }
         float* part = p.sp.o + (static_cast<long long>(blockIdx.y) * p.sp.rows + at) * a.d;
         __nv_bfloat16* out = static_cast<__nv_bfloat16*>(a.out) + b * a.os.b + (hk * group + g) * a.os.h + t * a.os.t;

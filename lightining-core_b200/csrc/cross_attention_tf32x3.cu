@@ -27,7 +27,6 @@ void* tensor_map_encoder();
 namespace {
 
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kLn2 = 0.6931471805599453f;
 constexpr int TILE = 128;
 constexpr int PIECE = 32768;     // hi and lo planes of a streamed tile
 constexpr int ACH = TILE * 128;  // one [128 rows x 32 fp32] swizzled chunk
@@ -360,6 +359,7 @@ __global__ void __launch_bounds__(FWD_THREADS, 1)
     const int quarter = warp & 3, half = warp >= 7 ? 1 : 0;
     const int row = quarter * 32 + lane;
     const uint32_t lanes = tmem + (static_cast<uint32_t>(quarter * 32) << 16);
+    const float floor = cross_floor(scale_log2);
     float m = -INFINITY, l = 0.0f, alpha_prev = 1.0f, o_acc[OC];
 #pragma unroll
     for (int e = 0; e < OC; ++e) o_acc[e] = 0.0f;
@@ -408,8 +408,10 @@ __global__ void __launch_bounds__(FWD_THREADS, 1)
       tc_fence_after();
       uint32_t r[32];
       tmem_ld32(lanes + F::S_COL + static_cast<uint32_t>(s * T + own), r);
+      float lowest = floor;  // of the maximum, unless none of these keys is visible
       if (partial) {
         const unsigned w = __ballot_sync(0xffffffffu, seen);
+        if (!w) lowest = -INFINITY;
 #pragma unroll
         for (int e = 0; e < 32; ++e)
           if (!((w >> e) & 1u)) r[e] = __float_as_uint(-INFINITY);
@@ -419,7 +421,7 @@ __global__ void __launch_bounds__(FWD_THREADS, 1)
       for (int i = 0; i < 4; ++i) mx4[i] = __uint_as_float(r[i]);
 #pragma unroll
       for (int e = 4; e < 32; ++e) mx4[e & 3] = fmaxf(mx4[e & 3], __uint_as_float(r[e]));
-      float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
+      float mx = fmaxf(fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])), lowest);
       if constexpr (D == 64) {
         // Slot [j & 1] is written again for tile j + 2 only after the partner published tile j + 1, which it does
         // after reading this one.  The verdict is made uniform: the tcgen05 accesses are warp-collective.
@@ -471,12 +473,12 @@ __global__ void __launch_bounds__(FWD_THREADS, 1)
     if (ok && rr < rows && t < q_end) {
       const bool empty = m == -INFINITY, split = sp.splits > 1;
       const long long at = (static_cast<long long>(b) * a.hq + hk * group) * a.q_len + rr;  // dense row
-      const float f = empty ? 0.0f : split ? 1.0f : 1.0f / l;
+      const float f = split ? 1.0f : cross_inverse(m, l);  // (without a key the sums are 0)
       if (half == 0) {
         if (split)
           sp.ml[static_cast<long long>(blockIdx.y) * sp.rows + at] = make_float2(m, empty ? 0.0f : l);
         else if (a.lse)
-          a.lse[at] = empty ? -INFINITY : (m + log2f(l)) * kLn2;
+          a.lse[at] = cross_lse(m, l);
       }
       float* out = split ? sp.o + (static_cast<long long>(blockIdx.y) * sp.rows + at) * a.d
                          : static_cast<float*>(a.out) + b * a.os.b + (hk * group + g) * a.os.h + t * a.os.t;
