@@ -497,11 +497,14 @@ __global__ void __launch_bounds__(Tile<DP, TT>::NT) cross_dkv_simt_kernel(CrossG
       if constexpr (DV) dv[i][c] = 0.0f;
     }
   const int b_hi = g.kv_shared ? a.batch : b0 + 1;
+  unsigned any = 0;  // bit i: an entry sees key rg + i * GL
   for (int b = b0; b < b_hi; ++b) {
     const int q_end = cross_len(a.q_lens, b, a.q_len), kv_end = cross_len(a.kv_lens, b, a.kv_len);
     if (k0 >= kv_end) continue;
     const unsigned char* mask = a.key_mask ? a.key_mask + static_cast<long long>(b) * a.kv_len : nullptr;
     const auto visible = [&](int j) { return k0 + j < kv_end && (!mask || mask[k0 + j]); };
+#pragma unroll
+    for (int i = 0; i < 4; ++i) any |= static_cast<unsigned>(visible(rg + i * L::GL)) << i;
     __syncthreads();
     if (tid < TT) seen[tid] = visible(tid);
     stage<T, DP, TT>(K, static_cast<const T*>(a.k) + b * a.ks.b + hk * a.ks.h, a.d, vec,
@@ -578,6 +581,14 @@ __global__ void __launch_bounds__(Tile<DP, TT>::NT) cross_dkv_simt_kernel(CrossG
       }
     }
   }
+  // A masked key's sums hold weights of 0 times rows that may be NaN or infinite.
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int c = 0; c < L::CPT; ++c) {
+      if constexpr (DK) dk[i][c] = (any >> i) & 1u ? dk[i][c] : 0.0f;
+      if constexpr (DV) dv[i][c] = (any >> i) & 1u ? dv[i][c] : 0.0f;
+    }
   const float one[4] = {1.0f, 1.0f, 1.0f, 1.0f}, scale[4] = {a.scale, a.scale, a.scale, a.scale};
   if constexpr (DK)
     store_rows<T, DP, TT>(static_cast<T*>(g.dk) + b0 * a.ks.b + hk * a.ks.h, dk, scale, a.d, rg, cg,

@@ -782,6 +782,11 @@ __global__ void __launch_bounds__(GRAD_THREADS, 1) cross_grad_f32_tc_kernel(cons
       }
       arrive(&st->o_free);
     }
+    // A masked key's sums, and those of a row that sees no key, hold weights of 0 times rows that may be NaN or infinite.
+    if (keys ? !seen : mine.x == -INFINITY) {
+#pragma unroll
+      for (int e = 0; e < 64; ++e) acc[e] = 0.0f;
+    }
     if (ok && keys && r < a.kv_len) {
       float* dk = static_cast<float*>(p.g.dk) + b * a.ks.b + hk * a.ks.h + r * a.ks.t;
       float* dv = static_cast<float*>(p.g.dv) + b * a.vs.b + hk * a.vs.h + r * a.vs.t;

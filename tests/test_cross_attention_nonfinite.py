@@ -183,3 +183,70 @@ def test_nan_rows_at_any_scale(gpu, name, scale):
     out, lse = _run(torch, c)
     assert bool(out[0].isnan().all()) and bool(lse[0].isnan().all())
     assert not bool(out[1:].any()) and bool((lse[1:] == -INF).all())
+
+
+def _grads(torch, c, out, lse):
+    mem, o = c.like(c.dout)
+    o.copy_(out)
+    g = c.backward(o, lse)
+    torch.cuda.synchronize()
+    return [x.clone() for x in g]
+
+
+def _masked_are_zero(torch, c, dk, dv):
+    gone = ~c.vis.any(0, keepdim=True) if c.shared else ~c.vis
+    gone = gone[:, None, :, None].expand_as(dk)
+    assert not bool(dk[gone].ne(0).any()) and not bool(dv[gone].ne(0).any())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name", BACKWARD)
+@pytest.mark.parametrize("value", [NAN, INF])
+def test_masked_keys_have_no_gradient(gpu, name, value):
+    """Whatever the computed rows of dout, or of q, hold: dk and dv of a masked key are 0."""
+    import torch
+    c = _case(torch, gpu, BACKWARD[name])
+    out, lse = _run(torch, c)
+    keep = c.dout.clone()
+    c.dout[0, :, c.nq // 3, 6] = value
+    dq, dk, dv = _grads(torch, c, out, lse)
+    _masked_are_zero(torch, c, dk, dv)
+    assert not bool(torch.isfinite(dv[0][:, c.vis[0], 6]).any())
+    c.dout.copy_(keep)
+    c.q[0, :, c.nq // 2, 1] = value
+    out, lse = _run(torch, c)
+    dq, dk, dv = _grads(torch, c, out, lse)
+    _masked_are_zero(torch, c, dk, dv)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name", BACKWARD)
+def test_rows_without_a_key_have_no_gradient(gpu, name):
+    """The batch entry without a visible key: NaN and infinities in its rows of q and dout reach nothing."""
+    import torch
+    c = _case(torch, gpu, BACKWARD[name])
+    out, lse = _run(torch, c)
+    want = _grads(torch, c, out, lse)
+    c.q[1] = NAN
+    c.dout[1] = INF
+    c.dout[1, :, 0] = NAN
+    again = _run(torch, c)
+    got = _grads(torch, c, *again)
+    assert torch.equal(again[0], out) and torch.equal(again[1], lse)
+    assert not any(bool(g[1].ne(0).any()) for g in got) and all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,d", [("bf16", 64), ("bf16", 128), ("bf16", 36), ("f32", 64), ("f32", 200)])
+@pytest.mark.parametrize("value", [NAN, INF])
+def test_a_shared_source(gpu, dtype, d, value):
+    """One source for the batch: keys that no entry sees have the gradient 0 whatever the rows hold."""
+    import torch
+    c = _case(torch, gpu, (dtype, "tokens", (3, 4, 2, 30, 200, d)), shared=True)
+    out, lse = _run(torch, c)
+    c.dout[0, 0, 2, 6] = value
+    dq, dk, dv = _grads(torch, c, out, lse)
+    _masked_are_zero(torch, c, dk, dv)
+    seen = c.vis[0]
+    assert not bool(torch.isfinite(dk[0, 0][seen]).any()) and not bool(torch.isfinite(dv[0, 0][seen][:, 6]).any())
+    assert not bool(torch.isfinite(dq[0, 0, 2]).any()) and bool(torch.isfinite(dq[1:]).all())
