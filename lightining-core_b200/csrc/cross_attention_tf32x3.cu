@@ -183,14 +183,17 @@ __device__ __forceinline__ void tmem_read(uint32_t at, uint32_t (&r)[N]) {
   else
     tmem_ld16(at, r);
 }
-// Hi and lo parts of 16 finite values into two groups of 16 columns (the tensor core ignores the 13 low bits).
+// Hi and lo parts of 16 values into two groups of 16 columns (the tensor core ignores the 13 low bits: half a unit is
+// added to the bits of hi, and 2^-11 of itself, half a unit to one, to lo: off by 2^-11 of lo at most either way).
+// The hi part of a NaN may be anything, as the carry reaches its sign; the lo part of a NaN and of an infinity is
+// NaN, which adding to the bits would lose and the multiplication keeps.
 __device__ __forceinline__ void put_split(uint32_t hi_at, uint32_t lo_at, const float* v) {
   uint32_t wh[16], wl[16];
 #pragma unroll
   for (int i = 0; i < 16; ++i) {
     const float h = __uint_as_float((__float_as_uint(v[i]) + 0x1000u) & 0xffffe000u);
     wh[i] = __float_as_uint(h);
-    wl[i] = __float_as_uint(v[i] - h) + 0x1000u;
+    wl[i] = __float_as_uint((v[i] - h) * 1.00048828125f);
   }
   tmem_st16(hi_at, wh);
   tmem_st16(lo_at, wl);

@@ -250,3 +250,62 @@ def test_a_shared_source(gpu, dtype, d, value):
     seen = c.vis[0]
     assert not bool(torch.isfinite(dk[0, 0][seen]).any()) and not bool(torch.isfinite(dv[0, 0][seen][:, 6]).any())
     assert not bool(torch.isfinite(dq[0, 0, 2]).any()) and bool(torch.isfinite(dq[1:]).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name", BACKWARD)
+@pytest.mark.parametrize("value", [NAN, INF, -INF])
+def test_a_gradient_of_the_output(gpu, name, value):
+    """One value of a row of dout: the row of dq, that column of dv and all of dk at the visible keys are not finite;
+    masked keys' gradients are 0, and what the row does not reach keeps its bits."""
+    import torch
+    c = _case(torch, gpu, BACKWARD[name])
+    out, lse = _run(torch, c)
+    wq, wk, wv = _grads(torch, c, out, lse)
+    h, t, col = c.hq - 1, c.nq // 3, 6
+    c.dout[0, h, t, col] = value
+    dq, dk, dv = _grads(torch, c, out, lse)
+    _masked_are_zero(torch, c, dk, dv)
+    seen, hk = c.vis[0], c.hk - 1
+    assert not bool(torch.isfinite(dq[0, h, t]).any())
+    assert not bool(torch.isfinite(dk[0, hk][seen]).any()) and not bool(torch.isfinite(dv[0, hk][seen][:, col]).any())
+    dq[0, h, t], dk[0, hk], dv[0, hk, :, col] = wq[0, h, t], wk[0, hk], wv[0, hk, :, col]
+    assert torch.equal(dq, wq) and torch.equal(dk, wk) and torch.equal(dv, wv)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name", BACKWARD)
+@pytest.mark.parametrize("value", [NAN, INF])
+def test_a_query_and_its_gradients(gpu, name, value):
+    """A row of q whose weights are NaN: its dq, and dk and dv of every visible key of its head."""
+    import torch
+    c = _case(torch, gpu, BACKWARD[name])
+    out, lse = _run(torch, c)
+    want = _grads(torch, c, out, lse)
+    h, t, hk = c.hq - 1, c.nq // 3, c.hk - 1
+    c.q[0, h, t, 1] = value
+    out, lse = _run(torch, c)
+    dq, dk, dv = _grads(torch, c, out, lse)
+    _masked_are_zero(torch, c, dk, dv)
+    assert bool(dq[0, h, t].isnan().all())
+    assert bool(dk[0, hk][c.vis[0]].isnan().all()) and bool(dv[0, hk][c.vis[0]].isnan().all())
+    dq[0, h, t], dk[0, hk], dv[0, hk] = want[0][0, h, t], want[1][0, hk], want[2][0, hk]
+    assert all(torch.equal(a, b) for a, b in zip((dq, dk, dv), want))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name", BACKWARD)
+def test_a_value_and_its_gradients(gpu, name):
+    """A NaN in a visible value: dq of the rows that read it and dk of all that they see; dv does not depend on it."""
+    import torch
+    c = _case(torch, gpu, BACKWARD[name])
+    out, lse = _run(torch, c)
+    want = _grads(torch, c, out, lse)
+    c.v[0, 0, _seen(c), 4] = NAN
+    out, lse = _run(torch, c)
+    dq, dk, dv = _grads(torch, c, out, lse)
+    _masked_are_zero(torch, c, dk, dv)
+    other = _others(torch, c)
+    assert bool(dq[~other].isnan().all()) and bool(dk[0, 0][c.vis[0]].isnan().all())
+    dk[0, 0] = want[1][0, 0]
+    assert torch.equal(dq[other], want[0][other]) and torch.equal(dk, want[1]) and torch.equal(dv, want[2])
