@@ -8,8 +8,9 @@
 //               as it lies
 //   O += P V    lane (g, c) reads keys 2c, 2c+1, 2c+8, 2c+9 at columns 8g..8g+7 and pairs keys with byte
 //               permutes; n-tile u then holds the columns 8g + u
-// P enters the product as the sum of two bf16 numbers (what rounding the first leaves goes into a second
-// product), so no precision is lost to it; scores, statistics and sums are fp32.
+// P enters the product as the sum of two bf16 numbers: its upper half, and what that leaves, rounded (by 2^-15 of P
+// at most), in a second product; scores, statistics and sums are fp32.  The second part is 2^-126 at least, which no
+// sum of finite values sees, so that both have P's sign and an infinite value gives an infinity in both products.
 // fp32, at most 8 rows, head_dim <= 128 (tiles of 4096 / D keys): the CUDA cores, 2 * D * rows FMAs a key against 8 * D
 // bytes, are faster than the bytes.  A quad takes a key's dot products (the rows of Q in shared memory), then every
 // lane four columns of O.
@@ -38,6 +39,7 @@ namespace lcb {
 namespace {
 
 constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLeast = 1.17549435e-38f;  // 2^-126
 constexpr int WARPS = 4;
 constexpr int ROWS = 16, ROWS_F32 = 8;
 constexpr int THREADS = (WARPS + 1) * 32;
@@ -293,9 +295,10 @@ __global__ void __launch_bounds__(THREADS, 2)
         for (int t = 0; t < 2; ++t) {
           const float p0 = exp2f(fmaf(s[t][2 * r], sc, -base)), p1 = exp2f(fmaf(s[t][2 * r + 1], sc, -base));
           sum += p0 + p1;
-          const uint32_t h = pack_bf16x2(p0, p1);
-          hi[t * 2 + r] = h;
-          lo[t * 2 + r] = pack_bf16x2(p0 - __uint_as_float(h << 16), p1 - __uint_as_float(h & 0xffff0000u));
+          const uint32_t u0 = __float_as_uint(p0), u1 = __float_as_uint(p1);
+          hi[t * 2 + r] = __byte_perm(u0, u1, 0x7632);
+          lo[t * 2 + r] = pack_bf16x2(fmaxf(p0 - __uint_as_float(u0 & 0xffff0000u), kLeast),
+                                      fmaxf(p1 - __uint_as_float(u1 & 0xffff0000u), kLeast));
         }
         l[r] = fmaf(l[r], keep, sum);
         if (__any_sync(0xffffffffu, keep != 1.0f))

@@ -309,3 +309,24 @@ def test_a_value_and_its_gradients(gpu, name):
     assert bool(dq[~other].isnan().all()) and bool(dk[0, 0][c.vis[0]].isnan().all())
     dk[0, 0] = want[1][0, 0]
     assert torch.equal(dq[other], want[0][other]) and torch.equal(dk, want[1]) and torch.equal(dv, want[2])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name", FORWARD)
+@pytest.mark.parametrize("value", [INF, -INF])
+def test_an_infinite_value(gpu, name, value):
+    """An infinity in a visible value: every weight is positive, so its column is that infinity (in f32 on the tensor
+    cores NaN); a second one of the other sign makes it NaN."""
+    import torch
+    c = _case(torch, gpu, FORWARD[name], spread=0.5)
+    want, want_lse = _run(torch, c)
+    c.v[0, 0, _seen(c), 7] = value
+    got, lse = _run(torch, c)
+    other = _others(torch, c)
+    column = got[~other][:, 7]
+    assert bool(column.isnan().all() if _split_infinities(name) else (column == value).all())
+    got[~other] = torch.where(torch.arange(c.d, device="cuda") == 7, want[~other], got[~other])
+    assert torch.equal(got, want) and torch.equal(lse, want_lse)
+    c.v[0, 0, int(c.vis[0].nonzero()[0]), 7] = -value
+    got, _ = _run(torch, c)
+    assert bool(got[~other][:, 7].isnan().all())
