@@ -174,6 +174,18 @@ struct Ring {
   // Every lane: waits for the current row; gives up after the common limit and records it (the row
   // is then wrong, the barriers of the group still meet).
   __device__ bool wait() { return warp_wait_poll(&full[s], phase, abort_flag, err, kErrNormLoadWait); }
+  // The leader, after a failed wait for the current row: the copies in flight land (for so long at most) before the
+  // block's sums take the ring's place or the block ends.  `rows`: from the current one on.
+  __device__ void drain(size_t rows) {
+    const uint64_t t0 = globaltimer_ns();
+    int at = s;
+    uint32_t ph = phase;
+    for (size_t k = rows - left; k; --k) {
+      while (!mbar_try_wait(&full[at], ph) && globaltimer_ns() - t0 < 100000000ull) {
+      }
+      if (++at == stages) at = 0, ph ^= 1u;
+    }
+  }
   __device__ const uint8_t* row(int i) const { return mem + (s * NB + i) * pitch + (ALIGNED ? 0u : lead[i]); }
   __device__ void step() {
     if (++s == stages) s = 0, phase ^= 1u;
@@ -427,7 +439,10 @@ __global__ void __launch_bounds__(kBwdWarps * 32, 1) ln_bwd_kernel(LnBwd a, Rows
     const float r = rstd;
     const uint64_t r2 = pk2(r, r), nm = pk2(-mean, -mean);
     if (row + hop < a.rows) mean = *(mp += hop), rstd = *(rp += hop);
-    ok = ring.wait() && ok;
+    if (!ring.wait()) {
+      if (ok && t == 0) ring.drain((a.rows - row + hop - 1) / hop);
+      ok = false;
+    }
     uint64_t h[kOwn / 2], w[kOwn / 2], p1[4] = {0, 0, 0, 0}, p2[4] = {0, 0, 0, 0};
     read_own<T, VEC, FULL, kOwn>(h, ring.row(0), t, step, nvec);
     read_own<T, VEC, FULL, kOwn>(w, ring.row(1), t, step, nvec);
