@@ -376,7 +376,8 @@ lcError_t lcCrossAttentionForward(const lcCrossAttentionDesc* desc, const void* 
  * (not all three).  dk and dv are written for every key (0 for masked ones) and sum over the query
  * heads of a key head and, when k and v are both broadcast over the batch, over the batch (one
  * [kv_heads, kv_len, head_dim] gradient); the other strides that would make two gradients share memory
- * are LC_INVALID_VALUE.  All sums are fp32 (or wider) in a fixed order: the same call gives the same
+ * are LC_INVALID_VALUE.  A gradient must not overlap an input or another gradient: inputs are read until the call
+ * ends (the same pointer is LC_INVALID_VALUE).  All sums are fp32 (or wider) in a fixed order: the same call gives the same
  * bits.  Device pointers, asynchronous on `stream`; allocates a stream-ordered workspace: 8 bytes a row and,
  * in f32, the halves, of q, dout and k transposed too (8 times the bytes of q and 6 times those of k at
  * head_dim 64 or 128). */

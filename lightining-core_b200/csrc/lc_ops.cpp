@@ -927,6 +927,15 @@ lcError_t lcCrossAttentionBackward(const lcCrossAttentionDesc* desc, const void*
   const lcError_t st = cross_args(desc, &a);
   if (st != LC_SUCCESS) return st;
   if (!dout || !q || !k || !v || !out || !lse || (!dq && !dk && !dv) || !dk != !dv) return LC_INVALID_VALUE;
+  // A gradient over an input, or over another one.
+  const void *const ins[] = {dout, q, k, v, out, lse}, *const grads[] = {dq, dk, dv};
+  for (int i = 0; i < 3; ++i) {
+    if (!grads[i]) continue;
+    for (const void* p : ins)
+      if (grads[i] == p) return LC_INVALID_VALUE;
+    for (int j = 0; j < i; ++j)
+      if (grads[i] == grads[j]) return LC_INVALID_VALUE;
+  }
   if (dq && !strides_disjoint(a.qs, desc->batch, desc->q_heads, desc->q_len, desc->head_dim)) return LC_INVALID_VALUE;
   g.kv_shared = desc->batch > 1 && a.ks.b == 0 && a.vs.b == 0;
   const size_t kv_batch = g.kv_shared ? 1 : desc->batch;
