@@ -350,7 +350,7 @@ typedef struct lcCrossAttentionDesc {
   const int32_t* q_lens;
   const int32_t* kv_lens;
   const uint8_t* key_mask;
-  float scale; /* of the scores; 0 = 1/sqrt(head_dim) */
+  float scale; /* of the scores, positive and below 2^127; 0 = 1/sqrt(head_dim) */
   lcDataType dtype;
 } lcCrossAttentionDesc;
 

@@ -838,7 +838,7 @@ static lcError_t cross_args(const lcCrossAttentionDesc* desc, CrossArgs* a) {
   if (d.batch == 0 || d.q_heads == 0 || d.kv_heads == 0 || d.q_len == 0 || d.kv_len == 0 || d.head_dim == 0 ||
       d.q_heads % d.kv_heads != 0)
     return LC_INVALID_VALUE;
-  if (!(d.scale >= 0.0f) || std::isinf(d.scale)) return LC_INVALID_VALUE;
+  if (!(d.scale >= 0.0f && d.scale < 0x1p127f)) return LC_INVALID_VALUE;  // (times log2 e it is a finite factor)
   if (!float_type(d.dtype) || d.head_dim > 256) return LC_NOT_SUPPORTED;
   const size_t lim = INT_MAX - 1024;  // room for an index to run past the end of a last tile
   if (d.batch > lim || d.q_heads > lim || d.q_len > lim || d.kv_len > lim || d.kv_heads > lim || d.batch > lim / d.q_heads ||
