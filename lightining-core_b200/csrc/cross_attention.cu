@@ -742,6 +742,11 @@ cudaError_t CrossSplitWork::begin_parts(const CrossArgs& a, long long n, cudaStr
   const size_t stats = (static_cast<size_t>(n) * sp.rows + 1) / 2 * 2;  // the sums start on a 16-byte boundary
   const cudaError_t e = workspace_alloc(
       ctx, &ws, stats * sizeof(float2) + static_cast<size_t>(n) * sp.rows * a.d * sizeof(float), s);
+  if (e == cudaErrorMemoryAllocation) {  // no room: in one part, which needs none
+    cudaGetLastError();
+    sp.splits = 1;
+    return cudaSuccess;
+  }
   if (e != cudaSuccess) return e;
   sp.ml = static_cast<float2*>(ws);
   sp.o = reinterpret_cast<float*>(sp.ml + stats);
