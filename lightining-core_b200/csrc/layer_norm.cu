@@ -174,17 +174,14 @@ struct Ring {
   // Every lane: waits for the current row; gives up after the common limit and records it (the row
   // is then wrong, the barriers of the group still meet).
   __device__ bool wait() { return warp_wait_poll(&full[s], phase, abort_flag, err, kErrNormLoadWait); }
-  // The leader, after a failed wait for the current row: the copies in flight land (for so long at most) before the
-  // block's sums take the ring's place or the block ends.  `rows`: from the current one on.
-  __device__ void drain(size_t rows) {
+  // The leader, when a wait has failed: the last copies land (0.1 s at most) before the block's sums take the ring's
+  // place or the block ends.  `rows`: all of the group's.
+  __device__ void drain(size_t rows) const {
     const uint64_t t0 = globaltimer_ns();
-    int at = s;
-    uint32_t ph = phase;
-    for (size_t k = rows - left; k; --k) {
-      while (!mbar_try_wait(&full[at], ph) && globaltimer_ns() - t0 < 100000000ull) {
+    const size_t issued = rows - left, n = stages;
+    for (size_t k = issued > n ? issued - n : 0; k < issued; ++k)
+      while (!mbar_try_wait(&full[k % n], (k / n) & 1) && globaltimer_ns() - t0 < 100000000ull) {
       }
-      if (++at == stages) at = 0, ph ^= 1u;
-    }
   }
   __device__ const uint8_t* row(int i) const { return mem + (s * NB + i) * pitch + (ALIGNED ? 0u : lead[i]); }
   __device__ void step() {
@@ -439,10 +436,7 @@ __global__ void __launch_bounds__(kBwdWarps * 32, 1) ln_bwd_kernel(LnBwd a, Rows
     const float r = rstd;
     const uint64_t r2 = pk2(r, r), nm = pk2(-mean, -mean);
     if (row + hop < a.rows) mean = *(mp += hop), rstd = *(rp += hop);
-    if (!ring.wait()) {
-      if (ok && t == 0) ring.drain((a.rows - row + hop - 1) / hop);
-      ok = false;
-    }
+    ok = ring.wait() && ok;
     uint64_t h[kOwn / 2], w[kOwn / 2], p1[4] = {0, 0, 0, 0}, p2[4] = {0, 0, 0, 0};
     read_own<T, VEC, FULL, kOwn>(h, ring.row(0), t, step, nvec);
     read_own<T, VEC, FULL, kOwn>(w, ring.row(1), t, step, nvec);
@@ -477,6 +471,10 @@ __global__ void __launch_bounds__(kBwdWarps * 32, 1) ln_bwd_kernel(LnBwd a, Rows
 #pragma unroll
     for (int k = 0; k < kOwn / 2; ++k) w[k] = fma2(h[k], c2, fma2(w[k], r2, c1));
     write_own<T, VEC, FULL, kOwn>(dx, w, t, step, nvec);
+  }
+  if (!ok && t == 0) {  // (rows from this group's first one on)
+    const size_t first = static_cast<size_t>(blockIdx.x) * rw.groups + group;
+    ring.drain((a.rows - first + hop - 1) / hop);
   }
   griddep_launch_dependents();
   if (!a.part) return;
