@@ -129,14 +129,15 @@ __device__ __forceinline__ bool mbar_try_wait(uint64_t* bar, uint32_t parity) {
 // Bounded wait for threads whose wake-up latency is not critical (TMA producers): between polls
 // the thread sleeps `ns` nanoseconds, leaving issue slots to the warps that do the math.
 __device__ __forceinline__ bool mbar_wait_bounded_backoff(uint64_t* bar, uint32_t parity, volatile int* abort_flag,
-                                                          unsigned* err_word, unsigned code, unsigned ns) {
+                                                          unsigned* err_word, unsigned code, unsigned ns,
+                                                          uint64_t limit_ns = LC_WAIT_TIMEOUT_NS) {
   if (mbar_try_wait(bar, parity)) return true;
   const uint64_t t0 = globaltimer_ns();
   while (true) {
     __nanosleep(ns);
     if (mbar_try_wait(bar, parity)) return true;
     if (*abort_flag) return false;
-    if (globaltimer_ns() - t0 > LC_WAIT_TIMEOUT_NS) {
+    if (globaltimer_ns() - t0 > limit_ns) {
       *abort_flag = 1;
       if (err_word) atomicCAS(err_word, 0u, code);
       return false;

@@ -1091,8 +1091,10 @@ __global__ void __launch_bounds__(Grad<D, KV>::THREADS, 1)
           seen |= j.r0() + row < cross_len(a.kv_lens, b, a.kv_len) &&
                   (!a.key_mask || a.key_mask[static_cast<long long>(b) * a.kv_len + min(j.r0() + row, a.kv_len - 1)]);
       }
-      // (These warps wait long: they sleep between polls and leave the issue slots to the others.)
-      ok = mbar_wait_bounded_backoff(&st->done[x % NA], (x / NA) & 1, abort_flag, p.err, kErrCrossSoftmaxWait, 40);
+      // These warps wait for a whole job: they sleep between polls and leave the issue slots to the others, and have a
+      // millisecond more for each item (0.8 us; a job of a shared source walks the rows of the whole batch).
+      const uint64_t limit = LC_WAIT_TIMEOUT_NS + 1000000ull * static_cast<unsigned>(j.count(p));
+      ok = mbar_wait_bounded_backoff(&st->done[x % NA], (x / NA) & 1, abort_flag, p.err, kErrCrossSoftmaxWait, 40, limit);
       if (!__all_sync(0xffffffffu, ok)) break;
       tc_fence_after();
       if (NX == 1 && ahead.job < p.jobs) place_rows(x + 1);
