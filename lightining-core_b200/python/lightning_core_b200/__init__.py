@@ -522,9 +522,10 @@ def _ptr(buf):
     return None if buf is None else buf.ptr
 
 
-def layer_norm_affine(x, gamma=None, beta=None, eps=1e-5, dtype: int = F32):
+def layer_norm_affine(x, gamma=None, beta=None, eps=1e-5, dtype: int = F32, param_dtype: int = F32):
     """Layer norm with weights over the last axis (lcLayerNormForward): host x (float32, or uint16 bf16
-    bits with dtype=BF16), float32 gamma / beta of the last axis' size (None: 1 / 0).
+    bits with dtype=BF16), gamma / beta of the last axis' size (None: 1 / 0; float32, or bf16 bits with
+    param_dtype=BF16).
     Returns (out, mean, rstd), the statistics float32 over the leading axes, for
     :func:`layer_norm_backward`."""
     x = _typed(x, "x", dtype)
@@ -532,36 +533,38 @@ def layer_norm_affine(x, gamma=None, beta=None, eps=1e-5, dtype: int = F32):
         raise ValueError("x must have a last axis and elements")
     cols = x.shape[-1]
     rows = x.size // cols
-    w = [None if t is None else _f32(t, "weight").reshape(-1) for t in (gamma, beta)]
+    w = [None if t is None else _typed(t, "weight", param_dtype).reshape(-1) for t in (gamma, beta)]
     if any(t is not None and t.size != cols for t in w):
         raise ValueError("gamma and beta must have the size of x's last axis")
     dx, dg, db = _device(x), _device(w[0]), _device(w[1])
     dy, stats = DeviceBuffer(x.nbytes), DeviceBuffer(8 * rows)
     check(lib.lcLayerNormForward(dx.ptr, _ptr(dg), _ptr(db), dy.ptr, stats.value, stats.value + 4 * rows, rows, cols, 0,
-                                 0, eps, dtype, F32, None), "layer_norm_affine")
+                                 0, eps, dtype, param_dtype, None), "layer_norm_affine")
     check(lib.lcDeviceSynchronize(), "sync")
     mean, rstd = stats.download((2, rows), np.float32)
     return dy.download(x.shape, x.dtype), mean.reshape(x.shape[:-1]), rstd.reshape(x.shape[:-1])
 
 
-def layer_norm_backward(dout, x, mean, rstd, gamma=None, dtype: int = F32):
+def layer_norm_backward(dout, x, mean, rstd, gamma=None, dtype: int = F32, param_dtype: int = F32):
     """Gradients of :func:`layer_norm_affine` (lcLayerNormBackward): returns (dx, dgamma, dbeta), dx of
-    x's type, the weights' gradients float32."""
+    x's type, the weights' gradients of the weights'."""
     x, dout = _typed(x, "x", dtype), _typed(dout, "dout", dtype)
     if x.ndim < 1 or x.size == 0 or dout.shape != x.shape:
         raise ValueError("dout must have x's shape")
     cols = x.shape[-1]
     rows = x.size // cols
     mean, rstd = (_f32(t, "statistics").reshape(-1) for t in (mean, rstd))
-    gamma = None if gamma is None else _f32(gamma, "gamma").reshape(-1)
+    gamma = None if gamma is None else _typed(gamma, "gamma", param_dtype).reshape(-1)
+    wt = np.uint16 if param_dtype == BF16 else np.float32
+    at = cols * np.dtype(wt).itemsize
     if mean.size != rows or rstd.size != rows or (gamma is not None and gamma.size != cols):
         raise ValueError("mean and rstd must have one value per row, gamma one per column")
     dd, dx, dm, dr, dg = (_device(t) for t in (dout, x, mean, rstd, gamma))
-    gx, gw = DeviceBuffer(x.nbytes), DeviceBuffer(8 * cols)
-    check(lib.lcLayerNormBackward(dd.ptr, dx.ptr, _ptr(dg), dm.ptr, dr.ptr, gx.ptr, gw.value, gw.value + 4 * cols, rows,
-                                  cols, 0, 0, 0, dtype, F32, None), "layer_norm_backward")
+    gx, gw = DeviceBuffer(x.nbytes), DeviceBuffer(2 * at)
+    check(lib.lcLayerNormBackward(dd.ptr, dx.ptr, _ptr(dg), dm.ptr, dr.ptr, gx.ptr, gw.value, gw.value + at, rows, cols, 0,
+                                  0, 0, dtype, param_dtype, None), "layer_norm_backward")
     check(lib.lcDeviceSynchronize(), "sync")
-    dgamma, dbeta = gw.download((2, cols), np.float32)
+    dgamma, dbeta = gw.download((2, cols), wt)
     return gx.download(x.shape, x.dtype), dgamma, dbeta
 
 
