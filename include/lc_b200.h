@@ -323,7 +323,9 @@ lcError_t lcLayerNormForward(const void* x, const void* gamma, const void* beta,
  *   dgamma[c] = sum over rows of dout * h,  dbeta[c] = sum over rows of dout
  * dx (dtype) and dgamma / dbeta (param_dtype, overwritten) may each be NULL, but not all three;
  * gamma NULL = 1.  The sums over rows are fp32 in a fixed order: the same call gives the same bits.
- * dx may be dout or x itself (with the same stride) and must not overlap them otherwise.  Device
+ * dx may be dout or x itself (with the same stride) and must not overlap them otherwise.  Rows of dout and x that
+ * do not start or end on a 16-byte boundary are copied from the boundary before to the one after them: up to 15 bytes
+ * before the first row and behind the last one are read, and not used.  Device
  * pointers, asynchronous on `stream`; strides as above.  Allocates a stream-ordered workspace when
  * dgamma or dbeta is wanted. */
 lcError_t lcLayerNormBackward(const void* dout, const void* x, const void* gamma, const float* mean,
@@ -359,15 +361,20 @@ typedef struct lcCrossAttentionDesc {
  * key is 0.  lse (fp32, dense [batch, q_heads, q_len], may be NULL) receives the log of each row's
  * sum of exp(scale * q k^T) (-infinity for a row without a visible key), which the backward pass needs.
  * A row with a visible score of NaN or +infinity, or with -infinity for all of them, is NaN, and its lse too.
- * f32: fp32 arithmetic (on the tensor cores each product is the sum of three of its operands' high and low
- * halves, off by 2^-22 of its magnitude at most; visible infinities come out as NaN there); bf16: fp32
- * accumulation and softmax statistics, weights rounded to bf16; head_dim <= 256.  k and v may be broadcast over the batch (batch stride 0 with the other strides set: one source
+ * f32: fp32 arithmetic.  On the tensor cores (head_dim <= 128 and more than a few rows to a key head) each product is
+ * the sum of three of its operands' high and low halves, off by 3 * 2^-22 of its magnitude at most, beside the rounding
+ * of the sums, and visible infinities come out as NaN.
+ * bf16: fp32 accumulation and softmax statistics.  On the tensor cores the weights are rounded to bf16 for their product
+ * with v (2^-8 of each at most); at head_dim 64 or 128 with at most 16 rows to a key head two bf16 numbers hold each
+ * weight (2^-15), on the CUDA cores one fp32 number, so the same row can differ by that much between calls of
+ * different shapes.
+ * head_dim <= 256.  k and v may be broadcast over the batch (batch stride 0 with the other strides set: one source
  * for many targets).  `out` must not overlap itself or the inputs.
  * Policy as lcAttentionForward (NULL: device pointers, asynchronous; the output postprocess must be
  * neutral).  Host tensors are dense; q_lens follows upload_q, kv_lens and key_mask follow
  * upload_k, lse follows download_out.  Stream-ordered workspaces: for few queries over many keys, which are
- * split along the keys, and in f32 for the halves (twice the bytes of q, k and v at head_dim 64 or 128; where
- * they do not fit, a slower path needs none). */
+ * split along the keys, and in f32 for the halves, twice the bytes of q, k and v (their columns padded to 64 or 128; k
+ * and v once for every batch entry, broadcast or not).  Where they do not fit, a slower path needs none. */
 lcError_t lcCrossAttentionForward(const lcCrossAttentionDesc* desc, const void* q, const void* k, const void* v,
                                   void* out, float* lse, const lcAttentionIoPolicy* policy, lcStream_t stream);
 
@@ -377,10 +384,16 @@ lcError_t lcCrossAttentionForward(const lcCrossAttentionDesc* desc, const void* 
  * heads of a key head and, when k and v are both broadcast over the batch, over the batch (one
  * [kv_heads, kv_len, head_dim] gradient); the other strides that would make two gradients share memory
  * are LC_INVALID_VALUE.  A gradient must not overlap an input or another gradient: inputs are read until the call
- * ends (the same pointer is LC_INVALID_VALUE).  All sums are fp32 (or wider) in a fixed order: the same call gives the same
- * bits.  Device pointers, asynchronous on `stream`; allocates a stream-ordered workspace: 8 bytes a row and,
- * in f32, the halves, of q, dout and k transposed too (8 times the bytes of q and 6 times those of k at
- * head_dim 64 or 128). */
+ * ends (the same pointer is LC_INVALID_VALUE).
+ * All sums are fp32 (or wider) in a fixed order: the same call gives the same bits.  Products as in the forward pass:
+ * in bf16 on the tensor cores the weights and the gradients of the scores are rounded to bf16 (2^-8 of each at most)
+ * for theirs; on the CUDA cores, which also take f32 gradients of a source that the batch shares, they are fp32.
+ * Where the batch shares its source, a NaN or an infinity in a computed row of q or dout may reach dk and dv of keys
+ * that only other entries see.
+ * Device pointers, asynchronous on `stream`; allocates a stream-ordered workspace: 8 bytes a row (with q_len rounded
+ * up to 128; in f32 on the tensor cores with a key head's rows rounded up to 64) and, in f32, the halves, of q, dout and
+ * k transposed too: 8 times the bytes of q and 6 times those of k (padded and counted as above).  Without room for the
+ * halves a slower path takes the call; without room for the rows' 8 bytes it is LC_OUT_OF_MEMORY. */
 lcError_t lcCrossAttentionBackward(const lcCrossAttentionDesc* desc, const void* dout, const void* q, const void* k,
                                    const void* v, const void* out, const float* lse, void* dq, void* dk, void* dv,
                                    lcStream_t stream);

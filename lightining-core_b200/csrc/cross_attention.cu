@@ -13,7 +13,7 @@
 // two inner products read 8 float4 for 64 FMAs.  Masked keys and rows past the end are staged as
 // zeros and their scores replaced, so what memory holds there never enters a sum.
 // Bound by shared-memory reads and issue slots.  B200, fp32: [4, 16, 333 x 1000, 64] 370 us (15 TFLOP/s), backward 782;
-// [4, 16, 333 x 1000, 200] 1486 us, backward 4500 (with tiles of 32 rows, 64 threads, 3560 and 16253: hence one buffer
+// [4, 16, 333 x 1000, 200] 1500 us, backward 4480 (with tiles of 32 rows, 64 threads, 3560 and 16253: hence one buffer
 // for two operands above 128 columns, which leaves room for tiles of 64).
 // Rows of the heads that share a key head form one list (row = head-in-group * q_len + token), so
 // a tile of few queries is filled by its group.
@@ -318,8 +318,8 @@ __global__ void __launch_bounds__(256) cross_combine_kernel(CrossArgs a, CrossSp
 // Row terms, negated so that they are addends: -D with D = dout . out, and minus the row's
 // log-sum-exp in the log2 domain.  Rows that are not computed or see no key get -infinity and 0:
 // every weight exp2(s - inf) is 0.  One warp to a row; rows of the workspace are padded to whole
-// tiles of 128 tokens.  (The walks' blocks do not come in beside these kernels' last ones: they took 8 us from
-// them that way.)
+// tiles of 128 tokens (the walks load 64 at a time).  (The walks' blocks do not come in beside these kernels' last ones:
+// they took 8 us from them that way.)
 template <typename T>
 __global__ void __launch_bounds__(256) cross_row_terms_kernel(CrossGradArgs g, float* neg_lse2, float* neg_d, int q_pad,
                                                               long long rows) {
@@ -720,9 +720,9 @@ cudaError_t bwd_any(const CrossGradArgs& g, cudaStream_t s) {
 
 // Splits a problem of `blocks` row tiles along its key tiles (of `tile` keys) when the blocks alone leave SMs idle: as
 // many parts as fill `per_sm` blocks to an SM, at least `least` key tiles each -- a part's fill, drain and join must
-// not cost more than it saves.  B200, bf16 (128 keys a tile): [1, 8, 64 x 4000, 128] 25 us split, 60 not; [2, 8, 512 x
-// 512, 64] 23 in parts of one tile, 16.6 whole.  fp32 (64 keys): [1, 8, 100 x 1000, 64] 21 us, 25 in parts of one tile,
-// 33 whole; on the CUDA cores [1, 8, 100 x 1000, 200] 118 in parts of one tile, 746 whole.
+// not cost more than it saves.  B200, bf16 (128 keys a tile): [1, 8, 64 x 4000, 128] 25 us split, 59 not; [2, 8, 512 x
+// 512, 64] 23 in parts of one tile, 15.4 whole.  fp32 (64 keys): [1, 8, 100 x 1000, 64] 21 us, 25 in parts of one tile,
+// 34 whole; on the CUDA cores [1, 8, 100 x 1000, 200] 78 in parts of one tile, 361 whole.
 cudaError_t CrossSplitWork::begin(const CrossArgs& a, long long blocks, int tile, int least, int per_sm, cudaStream_t s) {
   DeviceCtx* ctx = device_ctx();
   if (!ctx) return cudaErrorNoDevice;

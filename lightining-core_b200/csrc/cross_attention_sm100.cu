@@ -89,14 +89,15 @@ __device__ __forceinline__ void load_mask_bytes(const unsigned char* mask, int k
 // TMEM: S_A 0, S_B 128.  At head_dim 64 P_A 256, P_B 320, O_A 384, O_B 448, and S_h(j+1) is issued when S_h(j)
 // is in the softmax warps' registers; at 128 O_A 256, O_B 384 leave P_h (bf16 pairs) to lie over the first half
 // of S_h.  The products with the first 64 weights of a step start while the other 64 are formed (at 128 509 us
-// instead of 527 below).  O is rescaled only when a row's maximum grows by more than
+// instead of 527 over the same inputs).  O is rescaled only when a row's maximum grows by more than
 // 2^8 (the final division makes up for it).  P is rounded to bf16 for the second product, 2^-8 of a weight at most and
 // unbiased; the row's sum takes the unrounded weights.
 // Bound by the issue slots and dependent steps of the softmax warps: about 3500 cycles a pair of tiles at head_dim 64
 // (MUFU 2048 of them, the products 1130) and 4300 at 128, where S, P and the sums of a tile follow one another (2200).
-// B200: [16, 16, 512 x 2048 ragged, 64] 111 us, [8, 16/4, 2048 x 4096, 128] 509 us (1.08 PFLOP/s); the CUDA cores
-// took 1937 us and 22.6 ms.  At 64, one issuing warp and P over S took 127; one thread to a row (8 warps fewer) 116;
-// a fourth of the exponentials by a polynomial on the FMA pipes, which pays in the self attention kernel, 113.
+// B200, inputs not in L2: [16, 16, 512 x 2048 ragged, 64] 112 us, [8, 16/4, 2048 x 4096, 128] 580 us (0.95 PFLOP/s;
+// called again and again on the same inputs 517); the CUDA cores took 1937 us and 22.6 ms.  At 64, where this took 111, one
+// issuing warp and P over S took 127; one thread to a row (8 warps fewer) 116; a fourth of the exponentials by a
+// polynomial on the FMA pipes, which pays in the self attention kernel, 113.
 template <int D>
 struct Fwd {
   static constexpr int NCH = D / 64;
@@ -548,8 +549,9 @@ __global__ void __launch_bounds__(Fwd<D>::THREADS, 1)
 //   * three issuing warps, for S, dP and the sums, which order each other by barriers only
 //   * resident blocks that go from job to job: four more warps load the next job's rows and store
 //     the last one's sums meanwhile (two sets of TMEM columns where they fit)
-// B200, row terms included: [16, 16, 512 x 2048 ragged, 64] 261 us (blocks of one job with one chain of products:
-// 471), [4, 16/4, 1024 x 2048 ragged, 128] 185 us (266).
+// B200, row terms included: [16, 16, 512 x 2048 ragged, 64] 293 us with inputs that are not in L2, 261 called again and
+// again on the same (blocks of one job with one chain of products: 471), [4, 16/4, 1024 x 2048 ragged, 128] 212 and 189
+// (266).  The times of single steps below and in the launches are such repeated calls'.
 constexpr int QT = 64;         // rows of an item
 constexpr int QCH = QT * 128;  // one [64 rows x 64 bf16] box
 template <int D, bool KV>

@@ -1,11 +1,11 @@
 // Cross attention in strict fp32 on the tensor cores, head_dim <= 128: forward and backward.
 //
 // Every product by the 3xTF32 split: x = x_hi + x_lo, both rounded to tf32 (x_lo is off by 2^-22 |x| at most), x.y ~=
-// x_hi.y_hi + x_hi.y_lo + x_lo.y_hi (what is dropped is 2^-22 |x y|).  A pre-pass writes the operands' hi and lo
+// x_hi.y_hi + x_hi.y_lo + x_lo.y_hi (what is dropped is 2^-22 |x y|, so a product is off by 3 * 2^-22 |x y| at most).  A pre-pass writes the operands' hi and lo
 // planes, dense by (batch, key head) pair and padded to D columns: rows (of the group: head in the group * q_len +
 // token; or keys), and where a product sums over rows or keys their transpose, so that every operand is K-major
 // (tf32 has no other form).  Rows that are not computed and masked keys are written as zeros: what memory holds
-// there never enters a product.
+// there never enters a product.  (The planes of k and v are a batch entry's own, as its mask is, broadcast or not.)
 // Blocks own 128 rows or keys, one block to an SM, and stream tiles of T = 4096 / D of the other side: a tile's hi and
 // lo planes are always 32 KB.  Long accumulations in the tensor core drift (it truncates), so a tile's sums are
 // folded into fp32 registers, rounded to nearest.  Visible infinities give NaN (inf - inf in the split).
@@ -230,7 +230,7 @@ __device__ __forceinline__ void store_cols(float* out, const float* v, float f, 
 //               tagged shared-memory words and P_hi lies over S_j's columns; at D = 128 a tile has 32 keys, each
 //               warp reads them all and P_hi has columns of its own.
 // The tensor pipe bounds it: 1536 cycles a tile of 64 keys at D = 64.
-// B200, [4, 16, 333 x 1000, 64] with holes: 84 us, planes included (370 us on the CUDA cores); D = 128: 174 (698).
+// B200, [4, 16, 333 x 1000, 64] with holes: 82 us, planes included (370 us on the CUDA cores); D = 128: 174 (698).
 template <int D>
 struct Fwd {
   static constexpr int T = 4096 / D, VS = D == 64 ? 2 : 1, OC = D / 2;
@@ -506,8 +506,8 @@ __global__ void __launch_bounds__(FWD_THREADS, 1)
 //           sums are folded
 //   warps 2..9  X into TMEM, then two warps to a row: P, dS, and a tile's sums folded into registers
 // The tensor pipe bounds it: 96 steps of 32 cycles a tile of 64 rows for dk and dv at D = 64, 72 for dq.
-// B200, [4, 16, 333 x 1000, 64]: 232 us, planes included (782 on the CUDA cores), D = 128: 562 (1852); one row a pair
-// 123 (226); [2, 8, 77 x 300, 64] 27 (84).
+// B200, [4, 16, 333 x 1000, 64]: 232 us, planes included (782 on the CUDA cores), D = 128: 559 (1852); one row a pair
+// 112 (226); [2, 8, 77 x 300, 64] 27 (84).
 enum GradPass { kGradDq, kGradDkv, kGradDk, kGradDv };
 
 template <int D>

@@ -123,8 +123,8 @@ __device__ __forceinline__ void group_sync(int id, int threads) {
 // with a warp to a row, weights re-read and no ring; 54 us with a one-row register prefetch at 8
 // columns a lane, bound by issue slots; 45 us so, with 16 columns a lane and packed fp32 pairs.
 // A copy starts on a 16-byte boundary: rows that do not are copied from the boundary before them to
-// the one after them (never into another page) and read from there with scalar accesses: [5003, 1333]
-// fp32 27 us (floor 12).
+// the one after them (never into another page; with dx over x or dout the bytes of a neighbouring row may be
+// written meanwhile, and are not used) and read from there with scalar accesses: [5003, 1333] fp32 27 us (floor 12).
 constexpr int kFwdOwn = 32, kBwdOwn = 16;     // columns a lane
 constexpr int kBwdWarps = 16;                 // of a block
 constexpr int kMaxCols = 8192;                // 16 warps to a row (backward)
