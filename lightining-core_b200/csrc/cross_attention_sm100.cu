@@ -36,13 +36,6 @@ __device__ __forceinline__ void load_tile(uint8_t* dst, const CUtensorMap* map, 
   for (int c = 0; c < nch; ++c) tma_load_4d(dst + c * CH, map, c * 64, token, h, b, bar);
 }
 
-// Bounded drain of a copy already issued, so that no block leaves with TMA writes in flight.
-__device__ __forceinline__ void drain_bar(uint64_t* bar, uint32_t ph) {
-  const uint64_t t0 = globaltimer_ns();
-  while (!mbar_try_wait(bar, ph) && globaltimer_ns() - t0 < 100000000ull) {
-  }
-}
-
 // Zeroes the rows of a staged tile for which keep(row) is false (one warp).  Swizzling permutes
 // inside a row only.  The matrix unit multiplies a masked row by a weight of 0, which would keep a
 // NaN or an infinity that memory holds there.

@@ -198,12 +198,6 @@ __device__ __forceinline__ void put_split(uint32_t hi_at, uint32_t lo_at, const 
   tmem_st16(hi_at, wh);
   tmem_st16(lo_at, wl);
 }
-// After a failed wait: what is in flight lands before the block ends.
-__device__ __forceinline__ void drain_bar(uint64_t* bar, uint32_t ph) {
-  const uint64_t t0 = globaltimer_ns();
-  while (!mbar_try_wait(bar, ph) && globaltimer_ns() - t0 < 100000000ull) {
-  }
-}
 // Stores N columns from column c0 of one row, scaled.
 template <int N>
 __device__ __forceinline__ void store_cols(float* out, const float* v, float f, int c0, int d, bool vec) {
