@@ -87,7 +87,7 @@ __device__ __forceinline__ void load_mask_bytes(const unsigned char* mask, int k
 // unbiased; the row's sum takes the unrounded weights.
 // Bound by the issue slots and dependent steps of the softmax warps: about 3500 cycles a pair of tiles at head_dim 64
 // (MUFU 2048 of them, the products 1130) and 4300 at 128, where S, P and the sums of a tile follow one another (2200).
-// B200, inputs not in L2: [16, 16, 512 x 2048 ragged, 64] 112 us, [8, 16/4, 2048 x 4096, 128] 580 us (0.95 PFLOP/s;
+// B200, inputs not in L2: [16, 16, 512 x 2048 ragged, 64] 112 us, [8, 16/4, 2048 x 4096, 128] 585 us (0.94 PFLOP/s;
 // called again and again on the same inputs 517); the CUDA cores took 1937 us and 22.6 ms.  At 64, where this took 111, one
 // issuing warp and P over S took 127; one thread to a row (8 warps fewer) 116; a fourth of the exponentials by a
 // polynomial on the FMA pipes, which pays in the self attention kernel, 113.
@@ -542,8 +542,8 @@ __global__ void __launch_bounds__(Fwd<D>::THREADS, 1)
 //   * three issuing warps, for S, dP and the sums, which order each other by barriers only
 //   * resident blocks that go from job to job: four more warps load the next job's rows and store
 //     the last one's sums meanwhile (two sets of TMEM columns where they fit)
-// B200, row terms included: [16, 16, 512 x 2048 ragged, 64] 293 us with inputs that are not in L2, 261 called again and
-// again on the same (blocks of one job with one chain of products: 471), [4, 16/4, 1024 x 2048 ragged, 128] 212 and 189
+// B200, row terms included: [16, 16, 512 x 2048 ragged, 64] 296 us with inputs that are not in L2, 261 called again and
+// again on the same (blocks of one job with one chain of products: 471), [4, 16/4, 1024 x 2048 ragged, 128] 213 and 189
 // (266).  The times of single steps below and in the launches are such repeated calls'.
 constexpr int QT = 64;         // rows of an item
 constexpr int QCH = QT * 128;  // one [64 rows x 64 bf16] box
