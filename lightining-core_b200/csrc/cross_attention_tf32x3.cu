@@ -1,11 +1,12 @@
 // Cross attention in strict fp32 on the tensor cores, head_dim <= 128: forward and backward.
 //
 // Every product by the 3xTF32 split: x = x_hi + x_lo, both rounded to tf32 (x_lo is off by 2^-22 |x| at most), x.y ~=
-// x_hi.y_hi + x_hi.y_lo + x_lo.y_hi (what is dropped is 2^-22 |x y|, so a product is off by 3 * 2^-22 |x y| at most).  A pre-pass writes the operands' hi and lo
-// planes, dense by (batch, key head) pair and padded to D columns: rows (of the group: head in the group * q_len +
-// token; or keys), and where a product sums over rows or keys their transpose, so that every operand is K-major
-// (tf32 has no other form).  Rows that are not computed and masked keys are written as zeros: what memory holds
-// there never enters a product.  (The planes of k and v are a batch entry's own, as its mask is, broadcast or not.)
+// x_hi.y_hi + x_hi.y_lo + x_lo.y_hi (what is dropped is 2^-22 |x y|, so a product is off by 3 * 2^-22 |x y| at most).
+// A pre-pass writes the operands' hi and lo planes, dense by (batch, key head) pair and padded to D columns: rows (of
+// the group: head in the group * q_len + token; or keys), and where a product sums over rows or keys their transpose, so
+// that every operand is K-major (tf32 has no other form).  Rows that are not computed and masked keys are written as
+// zeros: what memory holds there never enters a product.  (The planes of k and v are a batch entry's own, as its mask is,
+// broadcast or not.)
 // Blocks own 128 rows or keys, one block to an SM, and stream tiles of T = 4096 / D of the other side: a tile's hi and
 // lo planes are always 32 KB.  Long accumulations in the tensor core drift (it truncates), so a tile's sums are
 // folded into fp32 registers, rounded to nearest.  Visible infinities give NaN (inf - inf in the split).
